@@ -276,6 +276,73 @@ int qmm_matmul_rmsnorm(int encoding, const qmm_gptq_config* cfg, const void* x, 
                        int64_t workspace_bytes, int flags, void* stream);
 
 /*
+ * The experts of a mixture-of-experts block (no counterpart in the reference's op set).  A routing gives each of `tokens` tokens `top` experts; pair p = top t + j is
+ * the j-th expert of token t:
+ *   ids     int32[tokens, top]   the expert of each pair, 0 .. experts - 1; any other value: none
+ *   weights fp32 [tokens, top]   what its result counts in the token's sum
+ *   offsets int32[experts + 1], order int32[tokens top]: the pairs sorted by expert, in rising order for each; those of expert e are order[offsets[e] .. offsets[e + 1]),
+ *           those without one come last.
+ * qmm_route_experts makes all four from a router's logits (fp32 or bf16, row t at logits + t stride values): the `top` largest scores of each token, equal ones by
+ * rising index, -0 equal to 0, NaN below everything.  The score is softmax(logits) or sigmoid(logits); with `bias` (fp32[experts], may be null) the choice is made on
+ * score + bias and the weight is that of the score alone.  renormalize: the weights are divided by their sum (a sum of 0: they are 0); all are multiplied by
+ * `scale`.  A token whose logits are all -inf gets weights of 0.  experts up to 1024, top up to 64.
+ * qmm_group_experts makes offsets and order from ids that come from elsewhere.
+ * Both give the same order in every call (no atomics decide a place).  Workspace: qmm_experts_group_workspace_bytes (0 up to 1024 pairs; top: of a token, 1 for
+ * qmm_group_experts).
+ */
+enum qmm_scoring { QMM_SOFTMAX = 0, QMM_SIGMOID = 1 };
+#define QMM_MAX_EXPERTS 1024
+#define QMM_MAX_TOP 64
+int64_t qmm_experts_group_workspace_bytes(int64_t pairs, int experts, int top);
+int qmm_route_experts(const void* logits, int logits_dtype, int64_t stride, int64_t tokens, int experts, int top, int scoring, const float* bias, int renormalize,
+                      float scale, int32_t* ids, float* weights, int32_t* offsets, int32_t* order, void* workspace, int64_t workspace_bytes, void* stream);
+int qmm_group_experts(const int32_t* ids, int64_t pairs, int experts, int32_t* offsets, int32_t* order, void* workspace, int64_t workspace_bytes, void* stream);
+
+typedef struct qmm_routing {
+    const int32_t* offsets;
+    const int32_t* order;
+    const int32_t* ids;
+    const float* weights; /* QMM_EXPERTS_SUM only */
+    int64_t tokens;
+    int32_t top, experts;
+} qmm_routing;
+
+/*
+ * Matrix products grouped by expert: y[p, n] = lhs[row of p] . dequant(rhs[expert of p])^T with the products of qmm_matmul (Q4_0: the lhs quantised to Q8_0).
+ *   QMM_EXPERTS_EACH    out[p, n] = y
+ *   QMM_EXPERTS_SWIGLU  out[p, n] = silu(y of rhs) * (y of rhs2)
+ *   QMM_EXPERTS_SUM     out[t, n] = residual[t, n] + sum over j of weights[top t + j] y[top t + j, n], in that order (residual: null, fp32 or bf16[tokens, n])
+ * rhs (and rhs2): the packed matrices uint8[n, k/epb*bpb] of one GGUF encoding, expert e at rhs + e expert_stride bytes (as a GGUF file holds them, and with a larger stride
+ * inside a tensor that holds gate and up of an expert side by side).  lhs fp32 or bf16, lhs_rows = tokens (a token's row serves its `top` pairs) or
+ * tokens top (a row for each pair).  out fp32, with QMM_FLAG_OUT_BF16 bf16.  Pairs without an expert get zeros (a sum leaves them out).  Only the experts that have rows are
+ * read; nothing is asked of the device on the way, so the call can be captured.
+ * The routing's arrays may hold anything: what is not a pair or an expert is left out, nothing is read or written out of range.
+ * Workspace: qmm_matmul_experts_workspace_bytes.
+ */
+enum qmm_experts_op { QMM_EXPERTS_EACH = 0, QMM_EXPERTS_SWIGLU = 1, QMM_EXPERTS_SUM = 2 };
+int64_t qmm_matmul_experts_workspace_bytes(int op, int encoding, int lhs_dtype, int64_t lhs_rows, int64_t tokens, int top, int experts, int64_t n, int64_t k, int flags);
+int qmm_matmul_experts(int op, int encoding, const qmm_routing* routing, const void* lhs, int lhs_dtype, int64_t lhs_rows, int64_t k, const void* rhs,
+                       int64_t expert_stride, const void* rhs2, int64_t expert_stride2, int64_t n, const void* residual, int residual_dtype, void* out, void* workspace,
+                       int64_t workspace_bytes, int flags, void* stream);
+
+/*
+ * Log probabilities of given tokens, entropy and the largest alternatives of rows of logits (fp32 or bf16, row i at logits + i stride values, `vocab` of them):
+ *   logprobs[i, c] = x[token] - log sum exp x,  tokens int32 or (tokens_i64) int64[rows, per_row]; a negative token: 0 (padding); one of vocab or more: NaN
+ *   entropy[i]     = - sum p log p
+ *   top_ids, top_logprobs [rows, top]: the `top` (0 .. 64) largest logits by falling value, equal ones by rising index, NaN below everything
+ * A row with a NaN or with +inf gives NaN; one of -inf only log probabilities of -inf and an entropy of 0.
+ * Workspace: qmm_logprobs_workspace_bytes.
+ * qmm_matmul_logprobs is the same of the logits lhs . dequant(rhs)^T (arguments as qmm_matmul; vocab = n), which are kept in the workspace, some rows at a time, and nowhere else.
+ */
+int64_t qmm_logprobs_workspace_bytes(int dtype, int64_t rows, int64_t vocab, int top);
+int qmm_logprobs(const void* logits, int dtype, int64_t stride, int64_t rows, int64_t vocab, const void* tokens, int tokens_i64, int per_row, int top, float* logprobs,
+                 float* entropy, int32_t* top_ids, float* top_logprobs, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t qmm_matmul_logprobs_workspace_bytes(int encoding, const qmm_gptq_config* cfg, int lhs_dtype, int64_t m, int64_t n, int64_t k, int top);
+int qmm_matmul_logprobs(int encoding, const qmm_gptq_config* cfg, const void* lhs, int lhs_dtype, int64_t m, int64_t k, const void* const* rhs, int n_rhs, int64_t n,
+                        const void* tokens, int tokens_i64, int per_row, int top, float* logprobs, float* entropy, int32_t* top_ids, float* top_logprobs, void* workspace,
+                        int64_t workspace_bytes, void* stream);
+
+/*
  * Test hook for the bit-exact integer check: raw int32 block sums
  * out[m, n, k/32] = sum_32 (q4 - 8) * q8 of Q8_0 lhs blocks (uint8[m, k/32*34])
  * against Q4_0 rhs blocks.

@@ -20,6 +20,15 @@ from .ops import (
     repack_weights,
     RepackedWeights,
 )
+from .experts import (
+    ExpertRouting,
+    group_experts,
+    qmatmul_experts,
+    qmatmul_experts_sum,
+    qmatmul_experts_swiglu,
+    route_experts,
+)
+from .scores import LogProbs, logprobs, qmatmul_logprobs
 from .weights import GGUFWeights, load_gptq_config, load_gptq_linear
 
 __all__ = [
@@ -33,6 +42,15 @@ __all__ = [
     "RepackedWeights",
     "qmatmul_rmsnorm",
     "qmatmul_swiglu",
+    "route_experts",
+    "group_experts",
+    "ExpertRouting",
+    "qmatmul_experts",
+    "qmatmul_experts_swiglu",
+    "qmatmul_experts_sum",
+    "logprobs",
+    "qmatmul_logprobs",
+    "LogProbs",
     "dequantize",
     "quantize",
     "quantize_gptq",

@@ -17,11 +17,19 @@ QMM_FLAG_W_BF16 = 1
 QMM_FLAG_ACT_Q8K = 2
 QMM_FLAG_OUT_BF16 = 4
 QMM_OP_MATMUL, QMM_OP_RMSNORM, QMM_OP_SWIGLU, QMM_OP_REPACKED = 0, 1, 2, 3
+QMM_SOFTMAX, QMM_SIGMOID = 0, 1
+QMM_EXPERTS_EACH, QMM_EXPERTS_SWIGLU, QMM_EXPERTS_SUM = 0, 1, 2
+QMM_MAX_EXPERTS, QMM_MAX_TOP = 1024, 64
 QMM_STATIC_SCRATCH_BYTES = 64 * 1024 * 1024
 
 
 class GptqConfig(C.Structure):
     _fields_ = [("bits", C.c_int32), ("group_size", C.c_int32), ("desc_act", C.c_int32), ("sym", C.c_int32)]
+
+
+class Routing(C.Structure):
+    _fields_ = [("offsets", C.c_void_p), ("order", C.c_void_p), ("ids", C.c_void_p), ("weights", C.c_void_p), ("tokens", C.c_int64), ("top", C.c_int32),
+                ("experts", C.c_int32)]
 
 
 _i64, _int, _vp = C.c_int64, C.c_int, C.c_void_p
@@ -59,6 +67,16 @@ SIGNATURES = {
     "qmm_matmul_rmsnorm_workspace_bytes": (_i64, [_int, _int, _i64, _i64, _i64, _int]),
     "qmm_matmul_rmsnorm": (_int, [_int, C.POINTER(GptqConfig), _vp, _int, _vp, C.c_float, _i64, _i64, C.POINTER(_vp), _int, _i64,
                                   _vp, _vp, _i64, _int, _vp]),
+    "qmm_experts_group_workspace_bytes": (_i64, [_i64, _int, _int]),
+    "qmm_route_experts": (_int, [_vp, _int, _i64, _i64, _int, _int, _int, _vp, _int, C.c_float, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "qmm_group_experts": (_int, [_vp, _i64, _int, _vp, _vp, _vp, _i64, _vp]),
+    "qmm_matmul_experts_workspace_bytes": (_i64, [_int, _int, _int, _i64, _i64, _int, _int, _i64, _i64, _int]),
+    "qmm_matmul_experts": (_int, [_int, _int, C.POINTER(Routing), _vp, _int, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _int, _vp, _vp, _i64, _int, _vp]),
+    "qmm_logprobs_workspace_bytes": (_i64, [_int, _i64, _i64, _int]),
+    "qmm_logprobs": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _int, _int, _int, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "qmm_matmul_logprobs_workspace_bytes": (_i64, [_int, C.POINTER(GptqConfig), _int, _i64, _i64, _i64, _int]),
+    "qmm_matmul_logprobs": (_int, [_int, C.POINTER(GptqConfig), _vp, _int, _i64, _i64, C.POINTER(_vp), _int, _i64, _vp, _int, _int, _int, _vp, _vp, _vp, _vp, _vp,
+                                   _i64, _vp]),
     "qmm_block_dots_q4_0": (_int, [_vp, _vp, _i64, _i64, _i64, _vp, _vp]),
 }
 
@@ -128,6 +146,9 @@ def call():
 
         native.setup([(enc, code, *((_BLOCKS[enc].elements_per_block, _BLOCKS[enc].block_size) if enc in _BLOCKS else (0, 0)))
                       for enc, code in _CODES.items()])
+        from .experts import ExpertRouting
+
+        native.routing(ExpertRouting)
         _call = native
     return _call
 

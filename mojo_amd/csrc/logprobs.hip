@@ -1,0 +1,396 @@
+// Log probabilities of given tokens, entropy and the largest alternatives of rows of logits, in one pass over them.
+//
+//   m = max x, S = sum exp(x - m), t = sum (x - m) exp(x - m):   log p(i) = x_i - m - log S,   H = log S - t / S
+//
+// The elements equal to the running maximum are counted (c) and kept out of the sum (s), so that S = c + s and log S = log1p(c - 1 + s): a row whose
+// largest value holds all but 1e-6 of the mass has a log probability of 1e-6, not of what fp32 leaves of 1 + 1e-6.  c is a number, so counting it takes no rounding either.
+// Parts of a row (lanes, wavefronts, workgroups) each have their (m, c, s, t) and are joined with exp(m_i - m).
+//
+// Alternatives.  A value that is among the `top` largest lies in one of the `top` runs of neighbouring values (four lanes' loads: 16 fp32 or 32 bf16 values) with the largest maxima, equal ones by
+// rising index.  So the pass leaves the maximum of every run in LDS (two DPP steps a load), and what follows looks for the largest of few: of 16 runs together,
+// of the runs of the chosen ones, of the values of the chosen runs.  A key is the value's bits in an order that integers compare right, above the index inverted: equal values by rising index, no two keys alike.
+// The time does not depend on the values, where a list that every larger value is put into takes a row in rising order apart.
+//
+// What bounds it: with many rows the loads (a row is read once; the chosen runs again, from L2).  With few, the way through two launches: parts of a row go to several workgroups until
+// they are enough for the part, and one workgroup a row joins them.
+#include <algorithm>
+
+#include "experts.h"
+
+namespace qmm {
+
+namespace {
+
+constexpr int kLpThreads = 512, kLpWaves = kLpThreads / 64;
+constexpr int kLpLoads = 4;           // 16-byte loads of a lane at once
+constexpr int kLpStep = kLpThreads * kLpLoads;  // loads of a workgroup at once
+constexpr int kLpRuns = 8192;         // runs of a workgroup at most (LDS: 32 KB)
+
+struct LpState {
+    float m, s, t;
+    int c;
+};
+
+typedef uint32_t lp_u4 __attribute__((ext_vector_type(4)));
+
+// Larger values have larger numbers; -0 is 0, NaN is below everything.  Never 0.
+__device__ __forceinline__ uint32_t order_of(float x) {
+    const uint32_t b = __float_as_uint(x + 0.0f);
+    return x != x ? 1u : (b & 0x80000000u) ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ uint64_t key_of(float x, uint32_t index) { return (uint64_t)order_of(x) << 32 | (uint32_t)~index; }
+__device__ __forceinline__ uint32_t index_of(uint64_t key) { return ~(uint32_t)key; }
+
+// exp(d), d <= 0
+__device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * 1.44269504088896f); }
+// what stands for -inf where it meets a factor of exp(-inf) = 0
+constexpr float kLpFloor = -150.0f;
+
+// b joins a.  (m = -inf: nothing but -inf so far, whose number does not matter.)
+__device__ __forceinline__ void join(LpState& a, const LpState& b) {
+    const bool more = b.m > a.m;
+    const LpState hi = more ? b : a, lo = more ? a : b;
+    a = hi;
+    if (lo.m == hi.m) {
+        a.c += lo.c;
+        a.s += lo.s;
+        a.t += lo.t;
+    } else {
+        const float d = fmaxf(lo.m - hi.m, kLpFloor), f = exp_of(d), n = (float)lo.c + lo.s;
+        a.s = fmaf(f, n, a.s);
+        a.t = fmaf(f, fmaf(d, n, lo.t), a.t);
+    }
+}
+__device__ __forceinline__ LpState from_lane(const LpState& a, int mask) {
+    return {__shfl_xor(a.m, mask), __shfl_xor(a.s, mask), __shfl_xor(a.t, mask), __shfl_xor(a.c, mask)};
+}
+__device__ __forceinline__ void wave_join(LpState& a) {
+#pragma unroll
+    for (int mask = 32; mask; mask >>= 1) {
+        const LpState b = from_lane(a, mask);
+        join(a, b);
+    }
+}
+
+__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int mask) {
+    return (uint64_t)(uint32_t)__shfl_xor((int)(v >> 32), mask) << 32 | (uint32_t)__shfl_xor((int)v, mask);
+}
+// One step of a bitonic sort over the lanes: the larger of a pair to the lane with (lane & mask) == 0, if `falling`.
+__device__ __forceinline__ void exchange(uint64_t& v, int lane, int mask, bool falling) {
+    const uint64_t o = shfl_xor64(v, mask);
+    const bool low = (lane & mask) == 0;
+    v = (v > o) == (low == falling) ? v : o;
+}
+__device__ __forceinline__ void sort64(uint64_t& v, int lane) {  // falling
+#pragma unroll
+    for (int size = 2; size <= 64; size *= 2)
+#pragma unroll
+        for (int mask = size / 2; mask; mask >>= 1) exchange(v, lane, mask, size == 64 || (lane & size) == 0);
+}
+// a: falling; reversed: another falling list, last entry first.  The 64 largest of both, falling.
+__device__ __forceinline__ void merge64(uint64_t& a, uint64_t reversed, int lane) {
+    a = a > reversed ? a : reversed;
+#pragma unroll
+    for (int mask = 32; mask; mask >>= 1) exchange(a, lane, mask, true);
+}
+
+// The lists of the workgroup's wavefronts (falling, one entry a lane) to one, in lists[0 .. 63] (visible to all afterwards).
+template <int WAVES>
+__device__ __forceinline__ void merge_waves(uint64_t& mine, uint64_t* lists, int wave, int lane) {
+    __syncthreads();  // (whoever still reads the lists of before)
+    lists[wave * 64 + lane] = mine;
+#pragma unroll
+    for (int half = WAVES / 2; half; half >>= 1) {
+        __syncthreads();
+        if (wave < half) {
+            merge64(mine, lists[(wave + half) * 64 + 63 - lane], lane);
+            lists[wave * 64 + lane] = mine;
+        }
+    }
+    __syncthreads();
+}
+__device__ __forceinline__ uint64_t shfl64(uint64_t v, int lane) { return (uint64_t)(uint32_t)__shfl((int)(v >> 32), lane) << 32 | (uint32_t)__shfl((int)v, lane); }
+// The `top` largest of key(0) .. key(count - 1) (0: none) first in lists[0 .. 63].  (key is called by whole wavefronts.)
+template <int WAVES, typename F>
+__device__ __forceinline__ void top_keys(int count, int top, uint64_t* lists, int wave, int lane, F&& key) {
+    uint64_t mine = 0;
+    for (int at = wave * 64; at < count; at += WAVES * 64) {
+        uint64_t v = key(min(at + lane, count - 1));
+        if (at + lane >= count) v = 0;
+        if (at == wave * 64) {
+            sort64(v, lane);
+            mine = v;
+        } else if (__any(v > shfl64(mine, top - 1))) {
+            sort64(v, lane);
+            merge64(mine, shfl64(v, 63 - lane), lane);
+        }
+    }
+    merge_waves<WAVES>(mine, lists, wave, lane);
+}
+
+// A row as 16-byte loads at multiples of 16 bytes: load v holds the values v * kPer - skew .. of the row; the first and the last one may hold fewer.
+template <typename T>
+struct LpRow {
+    static constexpr int kPer = 16 / sizeof(T);
+    const T* aligned;
+    int skew, vocab;
+    __device__ __forceinline__ LpRow(const T* row, int v) : vocab(v) {
+        skew = (int)(((uintptr_t)row & 15) / sizeof(T));
+        aligned = row - skew;
+    }
+    __device__ __forceinline__ int loads() const { return (skew + vocab + kPer - 1) / kPer; }
+    __device__ __forceinline__ bool whole(int v) const { return v * kPer >= skew && (v + 1) * kPer - skew <= vocab; }
+    // the values of load v; -inf for those that the row does not have
+    __device__ __forceinline__ void get(int v, float (&x)[kPer]) const {
+        lp_u4 raw;
+        if (whole(v)) {
+            raw = *(const lp_u4*)(aligned + (int64_t)v * kPer);
+        } else {
+            T e[kPer];
+#pragma unroll
+            for (int i = 0; i < kPer; i++) {
+                const int at = v * kPer + i - skew;
+                if constexpr (sizeof(T) == 4) e[i] = at >= 0 && at < vocab ? aligned[(int64_t)v * kPer + i] : -__builtin_inff();
+                else e[i] = at >= 0 && at < vocab ? aligned[(int64_t)v * kPer + i] : (T)0xff80;
+            }
+            __builtin_memcpy(&raw, e, 16);
+        }
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            if constexpr (sizeof(T) == 4) x[i] = __uint_as_float(raw[i]);
+            else x[i] = __uint_as_float((i & 1) ? raw[i >> 1] & 0xffff0000u : raw[i >> 1] << 16);
+        }
+    }
+    __device__ __forceinline__ float at(int64_t i) const { return load_f32(aligned, i + skew); }
+};
+
+struct LpOut {
+    const void* tokens;  // null: none
+    int wide, per_row;   // 64-bit tokens; tokens of a row
+    float *chosen, *entropy, *top_values;
+    int32_t* top_ids;
+    int top;
+};
+
+// What a row's state says.  lists: its `top` largest keys.
+template <typename T>
+__device__ __forceinline__ void finish_row(int64_t row_number, const LpRow<T>& row, const LpState& a, const uint64_t* lists, const LpOut& out) {
+    const float rest = (float)(a.c - 1) + a.s, log_total = log1pf(rest);
+    const bool none = a.m == -__builtin_inff() && !(a.s != a.s);  // no mass at all
+    const float bad = a.m == __builtin_inff() ? __builtin_nanf("") : 0.0f;
+    auto log_p = [&](float x) { return none ? -__builtin_inff() : (x - a.m) - log_total + bad; };
+    for (int i = threadIdx.x; i < out.per_row; i += (int)blockDim.x) {
+        const int64_t at = row_number * out.per_row + i, token = out.wide ? ((const int64_t*)out.tokens)[at] : ((const int32_t*)out.tokens)[at];
+        out.chosen[at] = token < 0 ? 0.0f : token >= row.vocab ? __builtin_nanf("") : log_p(row.at(token));
+    }
+    if (threadIdx.x == 0) out.entropy[row_number] = none ? 0.0f : log_total - a.t / ((float)a.c + a.s) + bad;
+    if ((int)threadIdx.x < out.top) {
+        const uint32_t id = index_of(lists[threadIdx.x]);
+        out.top_ids[row_number * out.top + threadIdx.x] = (int32_t)id;
+        out.top_values[row_number * out.top + threadIdx.x] = log_p(row.at(id));
+    }
+}
+
+// A part of a row: `per` loads (a multiple of four) of it; parts: workgroups of a row.  One: the row is finished here.
+template <typename T>
+__global__ __launch_bounds__(kLpThreads) void logprobs_kernel(const T* __restrict__ logits, int64_t stride, int vocab, int per, int parts, LpState* __restrict__ states,
+                                                              uint64_t* __restrict__ keys, LpOut out) {
+    constexpr int kPer = LpRow<T>::kPer, kRun = 4 * kPer;  // values of a load, of a run
+    extern __shared__ __attribute__((aligned(16))) float runs[];
+    __shared__ uint64_t lists[kLpThreads];
+    __shared__ LpState waves[kLpWaves];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), part = (int)blockIdx.y;
+    const int64_t row_number = blockIdx.x;
+    const LpRow<T> row(logits + row_number * stride, vocab);
+    const int first = part * per, end = min(first + per, row.loads());
+    const bool wanted = out.top > 0;
+
+    const int whole0 = row.skew ? 1 : 0, whole1 = min(end, (row.skew + vocab) / kPer);  // loads that the row fills
+    float m = -__builtin_inff(), s = 0.0f, t = 0.0f;
+    int c = 0;  // (m and c: of the wavefront; s and t: of the lane)
+    for (int v0 = first + wave * 64 * kLpLoads; v0 < end; v0 += kLpStep) {
+        float x[kLpLoads][kPer], most[kLpLoads];
+        if (v0 >= whole0 && v0 + 64 * kLpLoads <= whole1) {
+            // (inside the row: all loads are asked for together)
+            lp_u4 raw[kLpLoads];
+#pragma unroll
+            for (int j = 0; j < kLpLoads; j++) raw[j] = *(const lp_u4*)(row.aligned + (int64_t)(v0 + j * 64 + lane) * kPer);
+#pragma unroll
+            for (int j = 0; j < kLpLoads; j++)
+#pragma unroll
+                for (int i = 0; i < kPer; i++) {
+                    if constexpr (sizeof(T) == 4) x[j][i] = __uint_as_float(raw[j][i]);
+                    else x[j][i] = __uint_as_float((i & 1) ? raw[j][i >> 1] & 0xffff0000u : raw[j][i >> 1] << 16);
+                }
+        } else {
+#pragma unroll
+            for (int j = 0; j < kLpLoads; j++) {
+                const int v = v0 + j * 64 + lane;
+                if (v < end) row.get(v, x[j]);
+                else
+#pragma unroll
+                    for (int i = 0; i < kPer; i++) x[j][i] = -__builtin_inff();
+            }
+        }
+        float all = -__builtin_inff();
+#pragma unroll
+        for (int j = 0; j < kLpLoads; j++) {
+            most[j] = x[j][0];
+#pragma unroll
+            for (int i = 1; i < kPer; i++) most[j] = fmaxf(most[j], x[j][i]);
+            all = fmaxf(all, most[j]);
+        }
+        if (wanted) {
+            // the maximum of a run, four lanes, is in all of them; lane j of four keeps that of load j
+            float keep = 0.0f;
+#pragma unroll
+            for (int j = 0; j < kLpLoads; j++) {
+                float q = fmaxf(most[j], dpp_move<0xB1>(most[j]));
+                q = fmaxf(q, dpp_move<0x4E>(q));
+                keep = (lane & 3) == j ? q : keep;
+            }
+            const int run = ((v0 - first) >> 2) + (lane & 3) * 16 + (lane >> 2);
+            if (run * 4 < end - first) runs[run] = keep;
+        }
+        if (__any(all >= m)) {
+            // a new maximum, or one equal to it: rare once some steps have passed
+            float now = fmaxf(all, m);
+#pragma unroll
+            for (int mask = 32; mask; mask >>= 1) now = fmaxf(now, __shfl_xor(now, mask));
+            if (now > m) {
+                const float d = fmaxf(m - now, kLpFloor), f = exp_of(d), n = lane == 0 ? (float)c : 0.0f;  // (what was the maximum is none now)
+                t = f * fmaf(d, s + n, t);
+                s = f * (s + n);
+                m = now;
+                c = 0;
+            }
+#pragma unroll
+            for (int j = 0; j < kLpLoads; j++)
+#pragma unroll
+                for (int i = 0; i < kPer; i++) {
+                    const bool is = x[j][i] == m;
+                    c += (int)__popcll(__ballot(is));
+                    const float d = x[j][i] - m, e = is ? 0.0f : exp_of(d);
+                    s += e;
+                    t = fmaf(is ? 0.0f : fmaxf(d, kLpFloor), e, t);
+                }
+        } else {
+#pragma unroll
+            for (int j = 0; j < kLpLoads; j++)
+#pragma unroll
+                for (int i = 0; i < kPer; i++) {
+                    const float d = x[j][i] - m, e = exp_of(d);
+                    s += e;
+                    t = fmaf(fmaxf(d, kLpFloor), e, t);
+                }
+        }
+    }
+    LpState a{m, s, t, lane == 0 ? c : 0};
+    wave_join(a);
+    if (lane == 0) waves[wave] = a;
+    __syncthreads();
+    a = waves[0];
+#pragma unroll
+    for (int w = 1; w < kLpWaves; w++) join(a, waves[w]);
+    if (wanted) {
+        const int count = (end - first + 3) / 4;  // runs of this part
+        int chosen;
+        if (count > kLpThreads) {
+            // sixteen runs together, then the runs of the chosen sixteens
+            top_keys<kLpWaves>((count + 15) / 16, out.top, lists, wave, lane, [&](int i) {
+                float w = runs[16 * i];
+#pragma unroll
+                for (int j = 1; j < 16; j++) w = fmaxf(w, runs[min(16 * i + j, count - 1)]);
+                return key_of(w, (uint32_t)i);
+            });
+            const uint64_t sixteens = lists[lane];
+            chosen = min(out.top, (count + 15) / 16);
+            top_keys<kLpWaves>(chosen * 16, out.top, lists, wave, lane, [&](int i) {
+                const int run = (int)index_of(shfl64(sixteens, i >> 4)) * 16 + (i & 15);
+                return run < count ? key_of(runs[run], (uint32_t)run) : 0;
+            });
+        } else {
+            top_keys<kLpWaves>(count, out.top, lists, wave, lane, [&](int i) { return key_of(runs[i], (uint32_t)i); });
+        }
+        const uint64_t best = lists[lane];
+        chosen = min(out.top, count);
+        top_keys<kLpWaves>(chosen * kRun, out.top, lists, wave, lane, [&](int i) {
+            const int64_t at = (first + (int64_t)index_of(shfl64(best, i / kRun)) * 4) * kPer + i % kRun - row.skew;  // of the row
+            return at >= 0 && at < vocab && at < (int64_t)end * kPer - row.skew ? key_of(row.at(at), (uint32_t)at) : 0;
+        });
+    }
+    if (parts == 1) return finish_row(row_number, row, a, lists, out);
+    const int64_t place = row_number * parts + part;
+    if (threadIdx.x == 0) states[place] = a;
+    if ((int)threadIdx.x < out.top) keys[place * out.top + threadIdx.x] = lists[threadIdx.x];
+}
+
+// The parts of a row, in their order.
+constexpr int kLpJoinWaves = 4;
+template <typename T>
+__global__ __launch_bounds__(64 * kLpJoinWaves) void logprobs_join_kernel(const T* __restrict__ logits, int64_t stride, int vocab, int parts, const LpState* __restrict__ states,
+                                                                          const uint64_t* __restrict__ keys, LpOut out) {
+    __shared__ uint64_t lists[64 * kLpJoinWaves];
+    const int lane = threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+    const int64_t row_number = blockIdx.x;
+    const LpRow<T> row(logits + row_number * stride, vocab);
+    LpState a{-__builtin_inff(), 0.0f, 0.0f, 0};
+    for (int i = lane; i < parts; i += 64) {
+        const LpState b = states[row_number * parts + i];
+        join(a, b);
+    }
+    wave_join(a);
+    if (out.top > 0) {
+        uint64_t mine = 0;
+        for (int i = wave; i < parts; i += kLpJoinWaves) {
+            const int at = i == wave ? lane : 63 - lane;
+            const uint64_t v = at < out.top ? keys[(row_number * parts + i) * out.top + at] : 0;
+            if (i == wave) mine = v;
+            else merge64(mine, v, lane);
+        }
+        merge_waves<kLpJoinWaves>(mine, lists, wave, lane);
+    }
+    finish_row(row_number, row, a, lists, out);
+}
+
+struct LpPlan {
+    int per, parts;
+};
+// Workgroups a row: as few as make the runs of one fit its LDS, and until there are four for each compute unit, no part below eight steps of a workgroup's loads.
+LpPlan lp_plan(int dtype, int64_t rows, int64_t vocab, int top) {
+    const int64_t per_load = dtype == QMM_F32 ? 4 : 8, loads = (vocab + 2 * per_load - 2) / per_load;  // (of the worst alignment)
+    const int64_t fewest = (loads + 4 * kLpRuns - 1) / (4 * kLpRuns), enough = (4 * (int64_t)compute_units() + rows - 1) / rows, most = std::max<int64_t>(1, loads / (2 * kLpStep));
+    int64_t parts = std::max(fewest, std::min(enough, most));
+    const int64_t per = ((loads + parts - 1) / parts + 3) / 4 * 4;
+    parts = (loads + per - 1) / per;
+    return {(int)per, (int)parts};
+}
+
+template <typename T>
+hipError_t run_logprobs(const T* logits, int dtype, int64_t stride, int64_t rows, int64_t vocab, const LpOut& out, void* workspace, hipStream_t s) {
+    const LpPlan p = lp_plan(dtype, rows, vocab, out.top);
+    uint64_t* const keys = (uint64_t*)workspace;
+    LpState* const states = (LpState*)(keys + rows * p.parts * out.top);
+    const size_t lds = out.top > 0 ? (size_t)((p.per + 3) / 4) * 4 : 0;
+    logprobs_kernel<T><<<dim3((unsigned)rows, (unsigned)p.parts), dim3(kLpThreads), lds, s>>>(logits, stride, (int)vocab, p.per, p.parts, states, keys, out);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || p.parts == 1) return e;
+    logprobs_join_kernel<T><<<dim3((unsigned)rows), dim3(64 * kLpJoinWaves), 0, s>>>(logits, stride, (int)vocab, p.parts, states, keys, out);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+int64_t logprobs_workspace_bytes(int dtype, int64_t rows, int64_t vocab, int top) {
+    const LpPlan p = lp_plan(dtype, rows, vocab, top);
+    return p.parts == 1 ? 0 : rows * p.parts * ((int64_t)sizeof(LpState) + 8 * (int64_t)top);
+}
+
+hipError_t launch_logprobs(const void* logits, int dtype, int64_t stride, int64_t rows, int64_t vocab, const void* tokens, bool wide, int per_row, int top, float* chosen,
+                           float* entropy, int32_t* top_ids, float* top_values, void* workspace, hipStream_t s) {
+    const LpOut out{tokens, wide, per_row, chosen, entropy, top_values, top_ids, top};
+    return dtype == QMM_F32 ? run_logprobs((const float*)logits, dtype, stride, rows, vocab, out, workspace, s)
+                            : run_logprobs((const uint16_t*)logits, dtype, stride, rows, vocab, out, workspace, s);
+}
+
+}  // namespace qmm

@@ -30,7 +30,8 @@ struct Encoding {
     int64_t elements, bytes;  // of a block; 0 for GPTQ
 } g_encodings[kEncodings];
 int g_encoding_count = 0;
-PyObject *s_quant_method, *s_bits, *s_group_size, *s_desc_act, *s_sym, *s_gptq;
+PyObject *s_quant_method, *s_bits, *s_group_size, *s_desc_act, *s_sym, *s_gptq, *s_experts, *s_weights, *s_offsets, *s_order;
+PyObject* s_routing = nullptr;  // the class ExpertRouting
 
 const Encoding* encoding_of(PyObject* o) {
     for (int i = 0; i < g_encoding_count; i++)
@@ -399,6 +400,231 @@ PyObject* py_quantize_gptq(PyObject*, PyObject* const* a, Py_ssize_t count) {
     END_HANDLE_TH_ERRORS
 }
 
+// A GPU tensor of float32 or bfloat16 rows at equal distances: contiguous, or a view [rows, n] of wider ones.
+struct Rows {
+    const at::Tensor* t = nullptr;
+    int dtype;
+    int64_t n, count, stride;
+
+    bool open(PyObject* o) {
+        if (!THPVariable_CheckExact(o)) return false;
+        t = &THPVariable_Unpack(o);
+        if (!t->is_cuda() || t->dim() < 1 || t->numel() == 0 || (dtype = float_code(t->scalar_type())) < 0) return false;
+        n = stride = t->size(-1);
+        count = t->numel() / n;
+        if (!t->is_contiguous()) {
+            if (t->dim() != 2 || t->stride(1) != 1 || t->stride(0) < n) return false;
+            stride = t->stride(0);
+        }
+        return true;
+    }
+};
+
+bool int_of(PyObject* o, int64_t low, int64_t high, int64_t& v) {
+    if (!PyLong_CheckExact(o)) return false;
+    int overflow = 0;
+    v = PyLong_AsLongLongAndOverflow(o, &overflow);
+    return !overflow && v >= low && v <= high;
+}
+
+PyObject* tuple_of(at::Tensor* t, int count) {
+    PyObject* tuple = PyTuple_New(count);
+    if (!tuple) return nullptr;
+    for (int i = 0; i < count; i++) {
+        PyObject* item = Py_None;
+        if (t[i].defined()) item = THPVariable_Wrap(std::move(t[i]));
+        else Py_INCREF(item);
+        PyTuple_SET_ITEM(tuple, i, item);
+    }
+    return tuple;
+}
+
+// route(logits, top_k, scoring, renormalize, bias, scale): experts, weights, offsets, order
+PyObject* py_route(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    HANDLE_TH_ERRORS
+    if (count != 6) return none();
+    Rows x;
+    Call c;
+    int64_t top;
+    if (!x.open(a[0]) || !int_of(a[1], 1, QMM_MAX_TOP, top) || top > x.n || x.n > QMM_MAX_EXPERTS || !c.open(x.t) || !PyUnicode_CheckExact(a[2]) || !PyBool_Check(a[3]) ||
+        !PyFloat_CheckExact(a[5]))
+        return none();
+    const bool softmax = PyUnicode_CompareWithASCIIString(a[2], "softmax") == 0;
+    if (!softmax && PyUnicode_CompareWithASCIIString(a[2], "sigmoid") != 0) return none();
+    const float* bias = nullptr;
+    if (a[4] != Py_None) {
+        const at::Tensor* b = gpu_tensor(a[4], c.device);
+        if (!b || b->scalar_type() != at::kFloat || b->dim() != 1 || b->size(0) != x.n) return none();
+        bias = (const float*)b->data_ptr();
+    }
+    c10::SmallVector<int64_t, 6> sizes(x.t->sizes().begin(), x.t->sizes().end());
+    sizes.back() = top;
+    at::Tensor out[4] = {c.empty(sizes, at::kInt), c.empty(sizes, at::kFloat), c.empty({x.n + 1}, at::kInt), c.empty({x.count * top}, at::kInt)};
+    const int64_t need = qmm_experts_group_workspace_bytes(x.count * top, (int)x.n, (int)top);
+    c10::DataPtr ws = c.workspace(need);
+    int rc;
+    {
+        NoGil go;
+        rc = qmm_route_experts(x.t->data_ptr(), x.dtype, x.stride, x.count, (int)x.n, (int)top, softmax ? QMM_SOFTMAX : QMM_SIGMOID, bias, a[3] == Py_True,
+                               (float)PyFloat_AS_DOUBLE(a[5]), (int32_t*)out[0].data_ptr(), (float*)out[1].data_ptr(), (int32_t*)out[2].data_ptr(), (int32_t*)out[3].data_ptr(),
+                               ws.get(), need, c.stream);
+    }
+    if (rc != QMM_OK) return none();
+    return tuple_of(out, 4);
+    END_HANDLE_TH_ERRORS
+}
+
+struct Attr {  // an attribute of a Python object, held
+    PyObject* o;
+    Attr(PyObject* from, PyObject* name) : o(PyObject_GetAttr(from, name)) {
+        if (!o) PyErr_Clear();
+    }
+    ~Attr() { Py_XDECREF(o); }
+};
+
+// The matrices of a layer's experts, uint8[experts, N, row bytes], each contiguous.
+const at::Tensor* expert_matrices(const Encoding* e, PyObject* o, int64_t k, int64_t experts, int device) {
+    if (!THPVariable_CheckExact(o)) return nullptr;
+    const at::Tensor& t = THPVariable_Unpack(o);
+    if (!t.is_cuda() || t.device().index() != device || t.scalar_type() != at::kByte || t.dim() != 3 || t.size(0) != experts || t.size(1) <= 0 || e->elements <= 0 ||
+        k % e->elements || t.size(2) != k / e->elements * e->bytes || t.stride(2) != 1 || t.stride(1) != t.size(2) || t.stride(0) < t.size(1) * t.size(2))
+        return nullptr;
+    return &t;
+}
+
+// experts(op, encoding, lhs, rhs, rhs2, routing, residual, out_dtype)
+PyObject* py_experts(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    HANDLE_TH_ERRORS
+    if (count != 8) return none();
+    const Encoding* e = encoding_of(a[1]);
+    Call c;
+    int64_t op;
+    const int out_type = float_code(a[7]);
+    if (!int_of(a[0], 0, 2, op) || !weight_encoding(e) || e->code == QMM_GPTQ || !c.open_lhs(a[2]) || out_type < 0 || !s_routing || (PyObject*)Py_TYPE(a[5]) != s_routing) return none();
+    Attr ids_o(a[5], s_experts), weights_o(a[5], s_weights), offsets_o(a[5], s_offsets), order_o(a[5], s_order);
+    if (!ids_o.o || !weights_o.o || !offsets_o.o || !order_o.o) return none();
+    const at::Tensor *ids = gpu_tensor(ids_o.o, c.device), *weights = gpu_tensor(weights_o.o, c.device), *offsets = gpu_tensor(offsets_o.o, c.device), *order = gpu_tensor(order_o.o, c.device);
+    if (!ids || !weights || !offsets || !order || ids->scalar_type() != at::kInt || weights->scalar_type() != at::kFloat || offsets->scalar_type() != at::kInt ||
+        order->scalar_type() != at::kInt || ids->dim() < 1 || ids->numel() == 0 || weights->sizes() != ids->sizes() || order->numel() != ids->numel() || offsets->dim() != 1 ||
+        offsets->size(0) < 2 || offsets->size(0) > QMM_MAX_EXPERTS + 1)
+        return none();
+    const int64_t top = ids->size(-1), tokens = ids->numel() / top, experts = offsets->size(0) - 1;
+    const at::Tensor *w = expert_matrices(e, a[3], c.k, experts, c.device), *w2 = expert_matrices(e, a[4], c.k, experts, c.device);
+    if (top > QMM_MAX_TOP || !w || !w2 || w->size(1) != w2->size(1)) return none();
+    const int64_t n = w->size(1);
+    const void* residual = nullptr;
+    int residual_type = QMM_F32;
+    if (a[6] != Py_None) {
+        const at::Tensor* r = gpu_tensor(a[6], c.device);
+        if (!r || (residual_type = float_code(r->scalar_type())) < 0 || r->numel() != tokens * n || r->size(-1) != n) return none();
+        residual = r->data_ptr();
+    }
+    c10::SmallVector<int64_t, 6> sizes(ids->sizes().begin(), ids->sizes().end());
+    if (op == QMM_EXPERTS_SUM) sizes.back() = n;
+    else sizes.push_back(n);
+    at::Tensor out = c.empty(sizes, out_type == QMM_BF16 ? at::kBFloat16 : at::kFloat);
+    const int flags = out_type == QMM_BF16 ? QMM_FLAG_OUT_BF16 : 0;
+    const int64_t need = qmm_matmul_experts_workspace_bytes((int)op, e->code, c.dtype, c.m, tokens, (int)top, (int)experts, n, c.k, flags);
+    c10::DataPtr ws = c.workspace(need);
+    const qmm_routing routing{(const int32_t*)offsets->data_ptr(), (const int32_t*)order->data_ptr(), (const int32_t*)ids->data_ptr(), (const float*)weights->data_ptr(), tokens,
+                              (int32_t)top, (int32_t)experts};
+    int rc;
+    {
+        NoGil go;
+        rc = qmm_matmul_experts((int)op, e->code, &routing, c.lhs->data_ptr(), c.dtype, c.m, c.k, w->data_ptr(), w->stride(0), w2->data_ptr(), w2->stride(0), n, residual, residual_type,
+                                out.data_ptr(), ws.get(), need, flags, c.stream);
+    }
+    if (rc != QMM_OK) return none();
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// The tokens of rows of shape `lead`, and the results: logprobs, entropy, top_ids, top_logprobs
+struct Scores {
+    const at::Tensor* tokens;
+    int per_row;
+    at::Tensor out[4];
+
+    bool open(const Call& c, PyObject* o, at::IntArrayRef lead, int64_t top) {
+        tokens = gpu_tensor(o, c.device);
+        if (!tokens || (tokens->scalar_type() != at::kLong && tokens->scalar_type() != at::kInt)) return false;
+        const auto sizes = tokens->sizes();
+        if (sizes == lead) per_row = 1;
+        else if (sizes.size() == lead.size() + 1 && sizes.slice(0, lead.size()) == lead && sizes.back() > 0 && sizes.back() <= INT32_MAX) per_row = (int)sizes.back();
+        else return false;
+        out[0] = c.empty(sizes, at::kFloat);
+        out[1] = c.empty(lead, at::kFloat);
+        if (top > 0) {
+            c10::SmallVector<int64_t, 6> with(lead.begin(), lead.end());
+            with.push_back(top);
+            out[2] = c.empty(with, at::kInt);
+            out[3] = c.empty(with, at::kFloat);
+        }
+        return true;
+    }
+    int wide() const { return tokens->scalar_type() == at::kLong; }
+    void* at_(int i) const { return out[i].defined() ? out[i].data_ptr() : nullptr; }
+};
+
+// logprobs(logits, tokens, top_k): logprobs, entropy, top_ids, top_logprobs (the latter two None without alternatives)
+PyObject* py_logprobs(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    HANDLE_TH_ERRORS
+    if (count != 3) return none();
+    Rows x;
+    Call c;
+    Scores s;
+    int64_t top;
+    if (!x.open(a[0]) || !int_of(a[2], 0, QMM_MAX_TOP, top) || !c.open(x.t) || !s.open(c, a[1], x.t->sizes().slice(0, x.t->dim() - 1), top)) return none();
+    const int64_t need = qmm_logprobs_workspace_bytes(x.dtype, x.count, x.n, (int)top);
+    c10::DataPtr ws = c.workspace(need);
+    int rc;
+    {
+        NoGil go;
+        rc = qmm_logprobs(x.t->data_ptr(), x.dtype, x.stride, x.count, x.n, s.tokens->data_ptr(), s.wide(), s.per_row, (int)top, (float*)s.at_(0), (float*)s.at_(1), (int32_t*)s.at_(2),
+                          (float*)s.at_(3), ws.get(), need, c.stream);
+    }
+    if (rc != QMM_OK) return none();
+    return tuple_of(s.out, 4);
+    END_HANDLE_TH_ERRORS
+}
+
+// matmul_logprobs(encoding, config, lhs, rhs, tokens, top_k): as logprobs
+PyObject* py_matmul_logprobs(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    HANDLE_TH_ERRORS
+    if (count != 6) return none();
+    const Encoding* e = encoding_of(a[0]);
+    Call c;
+    Weights w;
+    Scores s;
+    int64_t top;
+    if (!weight_encoding(e) || !c.open_lhs(a[2]) || !read_weights(e, a[1], a[3], c.k, c.device, w) || !int_of(a[5], 0, QMM_MAX_TOP, top) ||
+        !s.open(c, a[4], c.lhs->sizes().slice(0, c.lhs->dim() - 1), top))
+        return none();
+    const int64_t need = qmm_matmul_logprobs_workspace_bytes(e->code, w.cfg_p, c.dtype, c.m, w.n, c.k, (int)top);
+    c10::DataPtr ws = c.workspace(need);
+    int rc;
+    {
+        NoGil go;
+        rc = qmm_matmul_logprobs(e->code, w.cfg_p, c.lhs->data_ptr(), c.dtype, c.m, c.k, w.ptrs, w.count, w.n, s.tokens->data_ptr(), s.wide(), s.per_row, (int)top, (float*)s.at_(0),
+                                 (float*)s.at_(1), (int32_t*)s.at_(2), (float*)s.at_(3), ws.get(), need, c.stream);
+    }
+    if (rc != QMM_OK) return none();
+    return tuple_of(s.out, 4);
+    END_HANDLE_TH_ERRORS
+}
+
+// routing(type): the class of the routings that `experts` takes
+PyObject* py_routing(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    if (count != 1 || !PyType_Check(a[0])) {
+        PyErr_SetString(PyExc_TypeError, "routing takes a type");
+        return nullptr;
+    }
+    Py_INCREF(a[0]);
+    Py_XDECREF(s_routing);
+    s_routing = a[0];
+    Py_RETURN_NONE;
+}
+
 // setup([(member, code, elements, bytes), ...]): the members of QuantizationEncoding
 PyObject* py_setup(PyObject*, PyObject* const* a, Py_ssize_t count) {
     if (count != 1 || !PyList_Check(a[0]) || PyList_GET_SIZE(a[0]) > kEncodings) {
@@ -432,6 +658,11 @@ PyMethodDef g_methods[] = {
     method<py_dequantize>("dequantize", "dequantize(encoding, config, tensors, dtype) -> tensor or None"),
     method<py_quantize>("quantize", "quantize(encoding, x) -> tensor or None"),
     method<py_quantize_gptq>("quantize_gptq", "quantize_gptq(config, w) -> 4 tensors or None"),
+    method<py_route>("route", "route(logits, top_k, scoring, renormalize, bias, scale) -> 4 tensors or None"),
+    method<py_experts>("experts", "experts(op, encoding, lhs, rhs, rhs2, routing, residual, out_dtype) -> tensor or None"),
+    method<py_logprobs>("logprobs", "logprobs(logits, tokens, top_k) -> 4 tensors or None"),
+    method<py_matmul_logprobs>("matmul_logprobs", "matmul_logprobs(encoding, config, lhs, rhs, tokens, top_k) -> 4 tensors or None"),
+    method<py_routing>("routing", "routing(type)"),
     {nullptr, nullptr, 0, nullptr},
 };
 
@@ -446,7 +677,11 @@ PyMODINIT_FUNC PyInit__call(void) {
     s_desc_act = PyUnicode_InternFromString("desc_act");
     s_sym = PyUnicode_InternFromString("sym");
     s_gptq = PyUnicode_InternFromString("gptq");
-    if (!s_quant_method || !s_bits || !s_group_size || !s_desc_act || !s_sym || !s_gptq) return nullptr;
+    s_experts = PyUnicode_InternFromString("experts");
+    s_weights = PyUnicode_InternFromString("weights");
+    s_offsets = PyUnicode_InternFromString("offsets");
+    s_order = PyUnicode_InternFromString("order");
+    if (!s_quant_method || !s_bits || !s_group_size || !s_desc_act || !s_sym || !s_gptq || !s_experts || !s_weights || !s_offsets || !s_order) return nullptr;
     PyObject* const module = PyModule_Create(&g_module);
     // the build's torch and Python: the loader looks for these bytes in the file before it loads it
     if (module && PyModule_AddStringConstant(module, "compiled_for", QMM_CALL_STAMP) < 0) {

@@ -9,6 +9,7 @@
 #include <atomic>
 #include <string>
 
+#include "experts.h"
 #include "qmm_internal.h"
 
 namespace qmm {
@@ -40,6 +41,9 @@ int hip_status(hipError_t e, const char* what) {
     if (e == hipSuccess) return QMM_OK;
     return fail(QMM_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
 }
+
+// of the experts' products: pairs of a token and an expert; rows and columns of an expert's matrix
+constexpr int64_t kMostPairs = 1 << 28, kMostExpertRows = 1 << 18, kMostExpertColumns = 1 << 20;
 
 bool aligned(const void* p, uintptr_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
 
@@ -1274,6 +1278,157 @@ int64_t qmm_preferred_workspace_bytes(int op, int encoding, const qmm_gptq_confi
         }
         default: return 0;
     }
+}
+
+int64_t qmm_experts_group_workspace_bytes(int64_t pairs, int experts, int top) {
+    if (pairs <= 0 || experts <= 0 || top <= 0) return 0;
+    return qmm::experts_group_workspace_bytes(pairs, experts, top);
+}
+
+int qmm_route_experts(const void* logits, int logits_dtype, int64_t stride, int64_t tokens, int experts, int top, int scoring, const float* bias, int renormalize, float scale,
+                      int32_t* ids, float* weights, int32_t* offsets, int32_t* order, void* workspace, int64_t workspace_bytes, void* stream) {
+    if (!logits || !ids || !weights || !offsets || !order) return fail(QMM_ERR_INVALID, "qmm_route_experts: null pointer");
+    if (logits_dtype != QMM_F32 && logits_dtype != QMM_BF16) return fail(QMM_ERR_INVALID, "qmm_route_experts: logits must be f32 or bf16");
+    if (experts < 1 || experts > QMM_MAX_EXPERTS || top < 1 || top > QMM_MAX_TOP || top > experts)
+        return fail(QMM_ERR_INVALID, "qmm_route_experts: %d of %d experts (1 .. %d experts, 1 .. %d of them)", top, experts, QMM_MAX_EXPERTS, QMM_MAX_TOP);
+    if (tokens < 1 || tokens * top > kMostPairs || stride < experts) return fail(QMM_ERR_INVALID, "qmm_route_experts: %lld tokens, stride %lld", (long long)tokens, (long long)stride);
+    if (scoring != QMM_SOFTMAX && scoring != QMM_SIGMOID) return fail(QMM_ERR_INVALID, "qmm_route_experts: unknown scoring %d", scoring);
+    const int64_t need = qmm::experts_group_workspace_bytes(tokens * top, experts, top);
+    if (need > 0 && (!workspace || workspace_bytes < need))
+        return fail(QMM_ERR_WORKSPACE, "qmm_route_experts: workspace of %lld bytes required, %lld given", (long long)need, (long long)workspace_bytes);
+    return hip_status(qmm::launch_route_experts(logits, logits_dtype, stride, tokens, experts, top, scoring == QMM_SIGMOID, bias, renormalize != 0, scale, ids, weights, offsets, order,
+                                                workspace, (hipStream_t)stream),
+                      "qmm_route_experts");
+}
+
+int qmm_group_experts(const int32_t* ids, int64_t pairs, int experts, int32_t* offsets, int32_t* order, void* workspace, int64_t workspace_bytes, void* stream) {
+    if (!ids || !offsets || !order) return fail(QMM_ERR_INVALID, "qmm_group_experts: null pointer");
+    if (experts < 1 || experts > QMM_MAX_EXPERTS || pairs < 1 || pairs > kMostPairs)
+        return fail(QMM_ERR_INVALID, "qmm_group_experts: %lld pairs, %d experts (1 .. %d)", (long long)pairs, experts, QMM_MAX_EXPERTS);
+    const int64_t need = qmm::experts_group_workspace_bytes(pairs, experts, 1);
+    if (need > 0 && (!workspace || workspace_bytes < need))
+        return fail(QMM_ERR_WORKSPACE, "qmm_group_experts: workspace of %lld bytes required, %lld given", (long long)need, (long long)workspace_bytes);
+    return hip_status(qmm::launch_group_experts(ids, pairs, experts, offsets, order, workspace, (hipStream_t)stream), "qmm_group_experts");
+}
+
+// The products' own share of the workspace, then (a sum) the results of the pairs.
+static int64_t experts_product_bytes(const qmm::ExpertCall& c) { return up256(qmm::experts_rows_workspace_bytes(c)); }
+
+int64_t qmm_matmul_experts_workspace_bytes(int op, int encoding, int lhs_dtype, int64_t lhs_rows, int64_t tokens, int top, int experts, int64_t n, int64_t k, int flags) {
+    int64_t epb, bpb;
+    if (tokens <= 0 || top <= 0 || experts <= 0 || n <= 0 || k <= 0 || lhs_rows <= 0 || !block_params(encoding, epb, bpb)) return 0;
+    qmm::ExpertCall c{encoding, nullptr, lhs_dtype, lhs_rows == tokens ? top : 1, lhs_rows, {nullptr, nullptr}, {0, 0}, op == QMM_EXPERTS_SWIGLU, n, k};
+    return experts_product_bytes(c) + (op == QMM_EXPERTS_SUM ? up256(tokens * top * n * 4) : 0);
+}
+
+int qmm_matmul_experts(int op, int encoding, const qmm_routing* routing, const void* lhs, int lhs_dtype, int64_t lhs_rows, int64_t k, const void* rhs, int64_t expert_stride,
+                       const void* rhs2, int64_t expert_stride2, int64_t n, const void* residual, int residual_dtype, void* out, void* workspace, int64_t workspace_bytes, int flags,
+                       void* stream) {
+    const bool gated = op == QMM_EXPERTS_SWIGLU, sum = op == QMM_EXPERTS_SUM;
+    if (op != QMM_EXPERTS_EACH && !gated && !sum) return fail(QMM_ERR_INVALID, "qmm_matmul_experts: unknown op %d", op);
+    if (!routing || !routing->offsets || !routing->order || !routing->ids || !lhs || !rhs || !out || (gated && !rhs2) || (sum && !routing->weights))
+        return fail(QMM_ERR_INVALID, "qmm_matmul_experts: null pointer");
+    int64_t epb, bpb;
+    if (encoding == QMM_Q8_0 || encoding == QMM_Q8_K || encoding == QMM_GPTQ || !block_params(encoding, epb, bpb))
+        return fail(QMM_ERR_INVALID, "qmm_matmul_experts: encoding %d is not a GGUF weight encoding", encoding);
+    const int64_t tokens = routing->tokens, top = routing->top, experts = routing->experts;
+    if (experts < 1 || experts > QMM_MAX_EXPERTS || top < 1 || top > QMM_MAX_TOP || tokens < 1 || tokens > kMostPairs / top)
+        return fail(QMM_ERR_INVALID, "qmm_matmul_experts: %lld tokens, %lld of %lld experts", (long long)tokens, (long long)top, (long long)experts);
+    if (n < 1 || n > kMostExpertRows || k < 1 || k > kMostExpertColumns || k % epb)
+        return fail(QMM_ERR_INVALID, "qmm_matmul_experts: N=%lld (1 .. %lld) K=%lld (a multiple of %lld up to %lld)", (long long)n, (long long)kMostExpertRows, (long long)k, (long long)epb,
+                    (long long)kMostExpertColumns);
+    if (lhs_dtype != QMM_F32 && lhs_dtype != QMM_BF16) return fail(QMM_ERR_INVALID, "qmm_matmul_experts: lhs dtype must be f32 or bf16");
+    if (lhs_rows != tokens && lhs_rows != tokens * top)
+        return fail(QMM_ERR_INVALID, "qmm_matmul_experts: %lld lhs rows for %lld tokens with %lld experts each", (long long)lhs_rows, (long long)tokens, (long long)top);
+    const int64_t matrix = n * (k / epb * bpb);
+    if (experts > 1 && (expert_stride < matrix || (gated && expert_stride2 < matrix)))
+        return fail(QMM_ERR_INVALID, "qmm_matmul_experts: matrices of %lld bytes, %lld apart", (long long)matrix, (long long)expert_stride);
+    if (flags & ~QMM_FLAG_OUT_BF16) return fail(QMM_ERR_INVALID, "qmm_matmul_experts: flags 0x%x", flags);
+    if (residual && (!sum || (residual_dtype != QMM_F32 && residual_dtype != QMM_BF16)))
+        return fail(QMM_ERR_INVALID, "qmm_matmul_experts: a residual (f32 or bf16) goes with QMM_EXPERTS_SUM");
+    if (!aligned(lhs, 16) || !aligned(out, flags & QMM_FLAG_OUT_BF16 ? 2 : 4)) return fail(QMM_ERR_INVALID, "qmm_matmul_experts: lhs must be 16-byte aligned");
+    const qmm::ExpertCall c{encoding, lhs, lhs_dtype, lhs_rows == tokens ? (int)top : 1, lhs_rows, {(const uint8_t*)rhs, (const uint8_t*)rhs2}, {expert_stride, expert_stride2}, gated, n, k};
+    const qmm::Routing r{routing->offsets, routing->order, routing->ids, routing->weights, (int)(tokens * top), (int)top, (int)experts};
+    const int64_t need = qmm_matmul_experts_workspace_bytes(op, encoding, lhs_dtype, lhs_rows, tokens, (int)top, (int)experts, n, k, flags);
+    if (need > 0 && (!workspace || workspace_bytes < need))
+        return fail(QMM_ERR_WORKSPACE, "qmm_matmul_experts: workspace of %lld bytes required, %lld given", (long long)need, (long long)workspace_bytes);
+    if (need > 0 && !aligned(workspace, 256)) return fail(QMM_ERR_INVALID, "qmm_matmul_experts: workspace must be 256-byte aligned");
+    const bool out_bf16 = flags & QMM_FLAG_OUT_BF16;
+    float* const y = sum ? (float*)((char*)workspace + experts_product_bytes(c)) : nullptr;
+    if (int rc = hip_status(qmm::launch_experts_rows(c, r, sum ? (void*)y : out, out_bf16 && !sum, workspace, (hipStream_t)stream), "qmm_matmul_experts")) return rc;
+    if (!sum) return QMM_OK;
+    return hip_status(qmm::launch_experts_combine(r, y, n, residual, residual_dtype, out, out_bf16, (hipStream_t)stream), "qmm_matmul_experts(sum)");
+}
+
+int64_t qmm_logprobs_workspace_bytes(int dtype, int64_t rows, int64_t vocab, int top) {
+    if (rows <= 0 || vocab <= 0 || top < 0) return 0;
+    return qmm::logprobs_workspace_bytes(dtype, rows, vocab, top);
+}
+
+// what both entries ask of their outputs
+static int check_logprobs(const char* name, int64_t rows, int64_t vocab, const void* tokens, int per_row, int top, const void* logprobs, const void* entropy, const void* top_ids,
+                          const void* top_logprobs) {
+    if (!entropy || (per_row > 0 && (!tokens || !logprobs)) || (top > 0 && (!top_ids || !top_logprobs))) return fail(QMM_ERR_INVALID, "%s: null pointer", name);
+    if (rows < 1 || rows > INT32_MAX || vocab < 1 || vocab > (1 << 30)) return fail(QMM_ERR_INVALID, "%s: %lld rows of %lld logits", name, (long long)rows, (long long)vocab);
+    if (per_row < 0 || top < 0 || top > QMM_MAX_TOP || top > vocab)
+        return fail(QMM_ERR_INVALID, "%s: %d tokens a row, %d alternatives of %lld (at most %d)", name, per_row, top, (long long)vocab, QMM_MAX_TOP);
+    return QMM_OK;
+}
+
+int qmm_logprobs(const void* logits, int dtype, int64_t stride, int64_t rows, int64_t vocab, const void* tokens, int tokens_i64, int per_row, int top, float* logprobs, float* entropy,
+                 int32_t* top_ids, float* top_logprobs, void* workspace, int64_t workspace_bytes, void* stream) {
+    if (!logits) return fail(QMM_ERR_INVALID, "qmm_logprobs: null pointer");
+    if (int rc = check_logprobs("qmm_logprobs", rows, vocab, tokens, per_row, top, logprobs, entropy, top_ids, top_logprobs)) return rc;
+    if (dtype != QMM_F32 && dtype != QMM_BF16) return fail(QMM_ERR_INVALID, "qmm_logprobs: logits must be f32 or bf16");
+    if (rows > 1 && stride < vocab) return fail(QMM_ERR_INVALID, "qmm_logprobs: rows of %lld logits, %lld apart", (long long)vocab, (long long)stride);
+    if (!aligned(logits, dtype == QMM_F32 ? 4 : 2)) return fail(QMM_ERR_INVALID, "qmm_logprobs: logits must be aligned to their type");
+    const int64_t need = qmm::logprobs_workspace_bytes(dtype, rows, vocab, top);
+    if (need > 0 && (!workspace || workspace_bytes < need))
+        return fail(QMM_ERR_WORKSPACE, "qmm_logprobs: workspace of %lld bytes required, %lld given", (long long)need, (long long)workspace_bytes);
+    if (need > 0 && !aligned(workspace, 16)) return fail(QMM_ERR_INVALID, "qmm_logprobs: workspace must be 16-byte aligned");
+    return hip_status(qmm::launch_logprobs(logits, dtype, stride, rows, vocab, tokens, tokens_i64 != 0, per_row, top, logprobs, entropy, top_ids, top_logprobs, workspace, (hipStream_t)stream),
+                      "qmm_logprobs");
+}
+
+// Rows of logits at a time: one GiB of them, a whole number of 256 where that is more.
+static int64_t logprobs_rows(int64_t m, int64_t n) {
+    const int64_t most = std::max<int64_t>(1, ((int64_t)1 << 28) / n);
+    return std::min(m, most > 256 ? most / 256 * 256 : most);
+}
+// logits, then what the product or the log probabilities of the part (the last one may be shorter) need
+static int64_t logprobs_scratch(int encoding, const qmm_gptq_config* cfg, int lhs_dtype, int64_t m, int64_t n, int64_t k, int top) {
+    const int64_t rows = logprobs_rows(m, n), last = m % rows ? m % rows : rows;
+    int64_t need = 0;
+    for (int64_t r : {rows, last}) need = std::max(need, std::max(preferred_matmul(encoding, cfg, lhs_dtype, r, n, k, 0), qmm::logprobs_workspace_bytes(QMM_F32, r, n, top)));
+    return up256(need);
+}
+
+int64_t qmm_matmul_logprobs_workspace_bytes(int encoding, const qmm_gptq_config* cfg, int lhs_dtype, int64_t m, int64_t n, int64_t k, int top) {
+    if (m <= 0 || n <= 0 || k <= 0 || top < 0) return 0;
+    return up256(logprobs_rows(m, n) * n * 4) + logprobs_scratch(encoding, cfg, lhs_dtype, m, n, k, top);
+}
+
+int qmm_matmul_logprobs(int encoding, const qmm_gptq_config* cfg, const void* lhs, int lhs_dtype, int64_t m, int64_t k, const void* const* rhs, int n_rhs, int64_t n, const void* tokens,
+                        int tokens_i64, int per_row, int top, float* logprobs, float* entropy, int32_t* top_ids, float* top_logprobs, void* workspace, int64_t workspace_bytes,
+                        void* stream) {
+    if (!lhs) return fail(QMM_ERR_INVALID, "qmm_matmul_logprobs: null pointer");
+    if (int rc = check_logprobs("qmm_matmul_logprobs", m, n, tokens, per_row, top, logprobs, entropy, top_ids, top_logprobs)) return rc;
+    if (k <= 0 || k > INT32_MAX || (lhs_dtype != QMM_F32 && lhs_dtype != QMM_BF16)) return fail(QMM_ERR_INVALID, "qmm_matmul_logprobs: K=%lld, lhs dtype %d", (long long)k, lhs_dtype);
+    const int64_t need = qmm_matmul_logprobs_workspace_bytes(encoding, cfg, lhs_dtype, m, n, k, top), rows = logprobs_rows(m, n), logits_bytes = up256(rows * n * 4);
+    if (!workspace || workspace_bytes < need)
+        return fail(QMM_ERR_WORKSPACE, "qmm_matmul_logprobs: workspace of %lld bytes required, %lld given", (long long)need, (long long)workspace_bytes);
+    if (!aligned(workspace, 256)) return fail(QMM_ERR_INVALID, "qmm_matmul_logprobs: workspace must be 256-byte aligned");
+    float* const logits = (float*)workspace;
+    char* const rest = (char*)workspace + logits_bytes;
+    for (int64_t r0 = 0; r0 < m; r0 += rows) {
+        const int64_t r = std::min(rows, m - r0);
+        if (int rc = qmm_matmul(encoding, cfg, (const char*)lhs + r0 * k * (lhs_dtype == QMM_F32 ? 4 : 2), lhs_dtype, r, k, rhs, n_rhs, n, logits, rest, workspace_bytes - logits_bytes, 0, stream))
+            return rc;
+        const hipError_t e = qmm::launch_logprobs(logits, QMM_F32, n, r, n, (const char*)tokens + r0 * per_row * (tokens_i64 ? 8 : 4), tokens_i64 != 0, per_row, top, logprobs + r0 * per_row,
+                                                  entropy + r0, top_ids + r0 * top, top_logprobs + r0 * top, rest, (hipStream_t)stream);
+        if (e != hipSuccess) return hip_status(e, "qmm_matmul_logprobs");
+    }
+    return QMM_OK;
 }
 
 }  // extern "C"

@@ -1,0 +1,547 @@
+// The experts' products on the matrix cores: weights packed as they lie in memory, unpacked between the matrix-core instructions, lhs rows gathered by the expert's list.
+//
+// One launch narrows every lhs row to fp16 once (a row's pieces in operand order, next to each other: [K / 64][fp32: hi, residual][8 pieces of 8 columns]); what an expert gets is picked by address, so a
+// token's row is not copied to each of its experts.  Then a workgroup of eight wavefronts takes up to 32 FM rows of one expert's run x 256 columns (gated: 128 of gate and the same 128 of up, whose
+// results meet in LDS): each wavefront unpacks the weights of its 32 columns, the lhs goes global -> LDS directly, a chunk of 64 columns at a time into three buffers that all share.  A load brings
+// eight rows x 128 bytes, lines as memory has them; which of a row's pieces a lane asks for is turned by the row, so that the operands (piece p of 32 rows) are read back without bank conflicts.
+//
+// The grid counts groups of rows as if every expert's last one were a group more: how many rows an expert has is known on the device only.  A workgroup looks for its group in the offsets
+// (a scan by one wavefront's lanes) and leaves if there is none; a group with few rows runs the body for as many.  Groups of one expert share its weights on one XCD.
+//
+// Arithmetic as in gemm_staged.hip: exact products of integer codes and fp16 values, fp32 sums, scales applied to the sums of a scale block.
+#include <algorithm>
+#include <type_traits>
+
+#include "experts.h"
+#include "staged_weights.h"
+
+namespace qmm {
+
+namespace {
+
+struct EgArgs {
+    const uint8_t* a16;    // [lhs rows][k / 64 rounded up to whole units][hi, fp32: residual] of 128 bytes
+    const uint8_t* sums;   // [lhs rows][units][32 bytes]: sums of 32 columns, eight hi and eight lo parts; Q4_0: eight block scales, zeros
+    const float* inv;      // [lhs rows]
+    const uint8_t* w[2];
+    int64_t stride[2];
+    int lhs_top, n, k, units, gated;
+    void* out;
+    int out_bf16;
+};
+
+// The weights of one wavefront.  Loads to LDS (kAsync), a unit ahead, or through registers (Q4_0, rows of any number of blocks at any even address).
+template <int ENC, bool CENTER>
+struct EgStaged : StagedOf<ENC, 16, CENTER> {
+    using Base = StagedOf<ENC, 16, CENTER>;
+    static constexpr bool kAsync = true, kQ8 = false;
+    static constexpr int kBufs = 2, kAhead = Base::kLoads;
+};
+struct EgQ40 : Q40Weights<1> {
+    static constexpr bool kAsync = false, kQ8 = true;
+    static constexpr int kBufs = 1, kAhead = 0;
+};
+template <int ENC, bool CENTER>
+using EgWeights = std::conditional_t<ENC == QMM_Q4_0, EgQ40, EgStaged<ENC == QMM_Q4_0 ? QMM_Q4_K : ENC, CENTER>>;
+
+constexpr int kEgWaves = 8, kEgBufs = 3, kEgChunks = 4;  // chunks of 64 columns in a unit of 256
+struct EgRow {
+    int64_t at;  // of the row's results, in values; -1: none
+    float inv;
+    int pad;
+};
+template <int ENC, int FM, bool HILO>
+struct EgLds {
+    using W = EgWeights<ENC, HILO>;
+    static constexpr int kPer = HILO ? 2 : 1, kChunk = FM * 4096 * kPer, kWeights = kEgWaves * W::kBufs * W::kStage, kSums = W::kMin || W::kQ8 ? 2 * FM * 1024 : 0;
+    static constexpr int kW = kEgBufs * kChunk, kS = kW + kWeights, kResultRow = 40, kResults = kEgWaves * 32 * std::min(FM, 2) * kResultRow * 4;
+    static constexpr int kInfo = std::max(kS + kSums, kResults), kBytes = kInfo + 32 * FM * (int)sizeof(EgRow);
+    static_assert(kBytes <= kLdsPerCu, "fits a compute unit");
+};
+
+template <int ENC, int FM, bool HILO, bool GATED>
+__device__ __forceinline__ void experts_tile(const EgArgs& p, const Routing& r, const ExpertRows& rows, int col_tile) {
+    using W = EgWeights<ENC, HILO>;
+    using L = EgLds<ENC, FM, HILO>;
+    constexpr int kPer = L::kPer, kTotal = FM * 4 * kPer, kLoads = (kTotal + kEgWaves - 1) / kEgWaves;  // loads of a chunk, of a wavefront
+    constexpr bool kHasSums = W::kMin || W::kQ8, kUnit = W::kQ8 || (W::kMin && HILO);                   // kUnit: a unit's sums apart from the running ones
+    constexpr int kAhead = W::kAhead + (kHasSums ? 1 : 0);
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), row = lane & 31, g = lane >> 5;
+    constexpr int kCols = GATED ? 128 : 256;
+    const int mat = GATED ? wave >> 2 : 0, n0 = col_tile * kCols + 32 * (GATED ? wave & 3 : wave);
+    EgRow* const info = (EgRow*)(smem + L::kInfo);
+    auto lhs_row = [&](int i) __attribute__((always_inline)) { return max(pair_at(r, rows.first + min(i, rows.count - 1)), 0) / p.lhs_top; };
+    if (threadIdx.x < 32 * FM) {
+        const int i = (int)threadIdx.x, pair = pair_at(r, rows.first + min(i, rows.count - 1));
+        info[i].at = i < rows.count && pair >= 0 ? (int64_t)pair * p.n : -1;
+        info[i].inv = p.inv[max(pair, 0) / p.lhs_top];
+    }
+    WeightTensors wt{p.w[mat] + rows.expert * p.stride[mat], nullptr, nullptr, p.n, p.k, 0};
+    const int units = p.units, last_chunk = units * kEgChunks - 1;
+    const uint32_t lds0 = lds_address(smem);
+
+    // this wavefront's loads of a chunk: number first + j of them, eight rows each; lane l asks for the piece that belongs at l & 7 of row l >> 3
+    const int first = min(wave * kLoads, kTotal - kLoads);
+    const uint8_t* src[kLoads];
+#pragma unroll
+    for (int j = 0; j < kLoads; j++) {
+        const int i = first + j, plane = i / (FM * 4), at_row = i % (FM * 4) * 8 + (lane >> 3), piece = (lane & 7) ^ ((at_row >> 1) & 7);
+        src[j] = p.a16 + (int64_t)lhs_row(at_row) * units * (512 * kPer) + plane * 128 + piece * 16;
+    }
+    auto issue_lhs = [&](int chunk, int buf) __attribute__((always_inline)) {
+        const int64_t at = (int64_t)min(chunk, last_chunk) * (128 * kPer);
+#pragma unroll
+        for (int j = 0; j < kLoads; j++) load16_to_lds(src[j] + at, (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds0 + buf * L::kChunk + (first + j) * 1024)));
+    };
+    const uint8_t* sums_src = nullptr;
+    const int sums_tile = wave % FM;
+    if constexpr (kHasSums) sums_src = p.sums + (int64_t)lhs_row(32 * sums_tile + row) * units * 32 + g * 16;
+    W w;
+    w.init(wt, n0, lane, smem + L::kW + wave * W::kBufs * W::kStage);
+    auto issue_ahead = [&](int unit, int buf) __attribute__((always_inline)) {
+        if constexpr (W::kAsync) unrolled<W::kAhead>([&](auto j) __attribute__((always_inline)) { w.template issue<decltype(j)::value>(unit, buf); });
+        if constexpr (kHasSums) load16_to_lds(sums_src + (int64_t)unit * 32, (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds0 + L::kS + (buf * FM + sums_tile) * 1024)));
+    };
+
+    float16v T[FM], P[FM], U[kUnit ? FM : 1];
+#pragma unroll
+    for (int a = 0; a < FM; a++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            T[a][i] = P[a][i] = 0.0f;
+            if constexpr (kUnit) U[a][i] = 0.0f;
+        }
+    const float16v zero16 = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    // where a lane's operands of the four steps of a chunk lie
+    uint32_t at_step[4];
+#pragma unroll
+    for (int t = 0; t < 4; t++) at_step[t] = row * 128 + (((2 * t + g) ^ ((row >> 1) & 7)) << 4);
+    half8 af[2][FM][kPer], b[2][W::kPlanes];
+    auto read_lhs = [&](int step, int slot, uint32_t base) __attribute__((always_inline)) {
+#pragma unroll
+        for (int a = 0; a < FM; a++)
+#pragma unroll
+            for (int q = 0; q < kPer; q++) af[slot][a][q] = *(const half8*)(smem + base + at_step[step] + (q * FM + a) * 4096);
+    };
+
+    if constexpr (!W::kAsync) w.load(0);
+    issue_ahead(0, 0);
+    issue_lhs(0, 0);
+    issue_lhs(1, 1);
+    wait_vmcnt<kLoads>();
+    __syncthreads();
+    issue_lhs(2, 2);
+    if constexpr (W::kAsync) w.open(0, 0);
+    else w.open();
+    read_lhs(0, 0, 0);
+    w.template step<0>(0, b[0]);
+    float d = 0.0f;
+    int buf = 0;  // of the current chunk
+    for (int u = 0; u < units; u++) {
+        const int next = min(u + 1, units - 1);
+        // (nobody reads the sums and weights of the unit before any more)
+        if constexpr (!W::kAsync) w.load(next);
+        issue_ahead(next, (u + 1) & 1);
+        float dmin = 0.0f, dnext = 0.0f;
+        half8 scales[FM];
+        if constexpr (W::kQ8) {
+#pragma unroll
+            for (int a = 0; a < FM; a++) scales[a] = *(const half8*)(smem + L::kS + ((u & 1) * FM + a) * 1024 + lane * 16);
+        } else {
+            dnext = w.scale(0);
+            if constexpr (W::kMin && !HILO) dmin = w.min_scale(0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        unrolled<16>([&](auto tt) __attribute__((always_inline)) {
+            constexpr int t = decltype(tt)::value, cur = t & 1, chunk = t / 4;
+            if constexpr (t % 4 == 3) {
+                // The next chunk has arrived (asked for two boundaries ago, before the chunk after it; where the next unit's weights were asked for since, they are younger too), and every
+                // wavefront has read this one's operands into registers: its buffer takes the chunk after the two that are there.  At a unit's end the weights are older than the chunk.
+                wait_vmcnt<kLoads + (chunk < 2 ? kAhead : 0)>();
+                __syncthreads();
+                issue_lhs(u * kEgChunks + chunk + 3, buf);
+                buf = buf == kEgBufs - 1 ? 0 : buf + 1;
+            }
+            read_lhs((t + 1) % 4, cur ^ 1, (uint32_t)(buf * L::kChunk));
+            if constexpr (W::kAsync) {
+                if constexpr (t + 1 == 16) w.open(next, (u + 1) & 1);
+            }
+            w.template before_step<t>();
+            // one row tile every three steps, the last at steps 14 and 15
+            constexpr int min_a = (t - 14 + 3 * (FM - 1)) / 3, min_at = 14 - 3 * (FM - 1);
+            constexpr bool min_now = W::kMin && t >= min_at && (t - min_at) % 3 == 0;
+            half8 sf;
+            if constexpr (min_now) sf = *(const half8*)(smem + L::kS + ((u & 1) * FM + min_a) * 1024 + lane * 16);
+            if constexpr (W::kMin && HILO && t < 5) {
+                if constexpr (t == 0) dmin = w.open_offsets();
+                else w.template add_offsets<t - 1>();
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (W::kQ8) {
+#pragma unroll
+                for (int a = 0; a < FM; a++)
+#pragma unroll
+                    for (int q = 0; q < kPer; q++) P[a] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af[cur][a][q], b[cur][0], t % 2 ? P[a] : zero16, 0, 0, 0);
+                if constexpr (t % 2 == 1) {
+                    // the scales of a block as a matrix: the row's scale in slot t / 2 times the weight's in the same slot
+                    const half8 dw = w.template scale_operand<t / 2>(0);
+#pragma unroll
+                    for (int a = 0; a < FM; a++) {
+                        const float16v S = __builtin_amdgcn_mfma_f32_32x32x16_f16(scales[a], dw, zero16, 0, 0, 0);
+#pragma unroll
+                        for (int i = 0; i < 16; i++) U[a][i] = t == 1 ? P[a][i] * S[i] : fmaf(P[a][i], S[i], U[a][i]);
+                        if constexpr (t == 15) {
+#pragma unroll
+                            for (int i = 0; i < 16; i++) T[a][i] += U[a][i];
+                            asm volatile("" : "+v"(T[a]));
+                        } else {
+                            asm volatile("" : "+v"(U[a]));
+                        }
+                    }
+                }
+            } else if constexpr (t == 0) {
+#pragma unroll
+                for (int a = 0; a < FM; a++) {
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        if constexpr (kUnit) T[a][i] += fmaf(d, P[a][i], U[a][i]);
+                        else T[a][i] = fmaf(d, P[a][i], T[a][i]);
+                    }
+                    asm volatile("" : "+v"(T[a]));
+#pragma unroll
+                    for (int pl = 0; pl < W::kPlanes; pl++)
+#pragma unroll
+                        for (int q = 0; q < kPer; q++) P[a] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af[cur][a][q], b[cur][pl], q || pl ? P[a] : zero16, 0, 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                d = dnext;
+            } else {
+#pragma unroll
+                for (int pl = 0; pl < W::kPlanes; pl++)
+#pragma unroll
+                    for (int q = 0; q < kPer; q++)
+#pragma unroll
+                        for (int a = 0; a < FM; a++) P[a] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af[cur][a][q], b[cur][pl], P[a], 0, 0, 0);
+            }
+            float16v M;
+            if constexpr (min_now) {
+                if constexpr (HILO) {
+                    M = __builtin_amdgcn_mfma_f32_32x32x16_f16(sf, w.offsets_lo(), zero16, 0, 0, 0);
+                    M = __builtin_amdgcn_mfma_f32_32x32x16_f16(sf, w.offsets_hi(), M, 0, 0, 0);
+                } else {
+                    M = __builtin_amdgcn_mfma_f32_32x32x16_f16(sf, w.min_operand(0), zero16, 0, 0, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    if constexpr (kUnit) U[min_a][i] = dmin * M[i];
+                    else T[min_a][i] = fmaf(dmin, M[i], T[min_a][i]);
+                }
+            }
+            if constexpr (!W::kAsync) {
+                if constexpr (t + 1 == 16) w.open();  // (the scales of the unit before are used up)
+            }
+            w.template step<(t + 1) % 16>(0, b[cur ^ 1]);
+            if constexpr (!W::kQ8 && t != 0) {
+                constexpr int kMfma = FM * kPer * W::kPlanes, kValu = (W::kPlanes == 2 ? 28 : 12) + (min_now ? 16 : 0);  // spread evenly
+                unrolled<kMfma + (min_now ? (HILO ? 2 : 1) : 0)>([&](auto) __attribute__((always_inline)) {
+                    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x2, (kValu + kMfma - 1) / kMfma, 0);
+                });
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    }
+    if constexpr (!W::kQ8) {
+#pragma unroll
+        for (int a = 0; a < FM; a++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) T[a][i] = kUnit ? T[a][i] + fmaf(d, P[a][i], U[a][i]) : fmaf(d, P[a][i], T[a][i]);
+    }
+    wait_vmcnt<0>();
+    __syncthreads();  // nothing is on its way into the buffers any more, which now take the results
+    constexpr int kRow = L::kResultRow, kTiles = std::min(FM, 2), kTile = 32 * kTiles * kRow;
+    float* const mine = (float*)smem + wave * kTile;
+#pragma unroll
+    for (int a0 = 0; a0 < FM; a0 += kTiles) {
+        if (a0) __syncthreads();
+#pragma unroll
+        for (int a = a0; a < FM && a < a0 + kTiles; a++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) mine[(32 * (a - a0) + 8 * (i >> 2) + 4 * g + (i & 3)) * kRow + row] = T[a][i];
+        __syncthreads();
+        // two rows of 32 columns at a time; gated: the wavefronts of gate take the first half of the rows, those of up the second
+        const int strip = GATED ? wave & 3 : wave, col = col_tile * kCols + 32 * strip + row;
+        const float* const y = (const float*)smem + strip * kTile;
+        constexpr int kMine = GATED ? 16 * kTiles : 32 * kTiles;
+        const int from = GATED ? (wave >> 2) * kMine : 0;
+        if (col < p.n) {
+            for (int i0 = from + g; i0 < from + kMine; i0 += 8) {
+                EgRow e[4];
+                float v[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int i = i0 + 2 * j;
+                    e[j] = info[32 * a0 + i];
+                    v[j] = y[i * kRow + row] * e[j].inv;
+                    if constexpr (GATED) v[j] = v[j] / (1.0f + expf(-v[j])) * (y[4 * kTile + i * kRow + row] * e[j].inv);
+                }
+                if (p.out_bf16) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        if (e[j].at >= 0) ((uint16_t*)p.out)[e[j].at + col] = f2bf(v[j]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        if (e[j].at >= 0) ((float*)p.out)[e[j].at + col] = v[j];
+                }
+            }
+        }
+    }
+}
+
+template <bool GATED>
+__device__ __forceinline__ void zero_tile(const EgArgs& p, const Routing& r, const ExpertRows& rows, int col_tile) {
+    constexpr int kCols = GATED ? 128 : 256;
+    const int col = col_tile * kCols + (int)threadIdx.x % kCols;
+    if (col >= p.n) return;
+    for (int i = (int)threadIdx.x / kCols; i < rows.count; i += 64 * kEgWaves / kCols) {
+        const int pair = pair_at(r, rows.first + i);
+        if (pair < 0) continue;
+        if (p.out_bf16) ((uint16_t*)p.out)[(int64_t)pair * p.n + col] = 0;
+        else ((float*)p.out)[(int64_t)pair * p.n + col] = 0.0f;
+    }
+}
+
+template <int ENC, int FM, bool HILO, bool GATED>
+__global__ __launch_bounds__(64 * kEgWaves, 2) void experts_gemm_kernel(EgArgs p, Routing r) {
+    const ExpertRows rows = find_rows<32 * FM>(r, (int)blockIdx.y, threadIdx.x & 63);
+    if (rows.count == 0) return;
+    // columns of one expert go over the XCDs, beginning with another one for each
+    const int col_tile = (int)blockIdx.z * 8 + (((int)blockIdx.x + rows.expert) & 7);
+    if (col_tile * (GATED ? 128 : 256) >= p.n) return;
+    if (rows.expert >= r.experts) return zero_tile<GATED>(p, r, rows, col_tile);
+    if constexpr (FM > 2) {
+        if (rows.count > 64) return experts_tile<ENC, FM, HILO, GATED>(p, r, rows, col_tile);
+    }
+    if constexpr (FM > 1) {
+        if (rows.count > 32) return experts_tile<ENC, 2, HILO, GATED>(p, r, rows, col_tile);
+    }
+    experts_tile<ENC, 1, HILO, GATED>(p, r, rows, col_tile);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------
+// the lhs
+// ---------------------------------------------------------------------------------------------------------------------------
+// A row by TPR threads, eight columns a thread and turn.
+template <typename AT, int TPR>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void experts_prep_kernel(const AT* __restrict__ a, int64_t rows, int k, int units, int with_sums, uint8_t* __restrict__ a16,
+                                                                             uint8_t* __restrict__ sums, float* __restrict__ inv) {
+    constexpr bool kF32 = sizeof(AT) == 4;
+    constexpr int kThreads = TPR > 256 ? TPR : 256, kPer = kF32 ? 2 : 1, kHeld = 4;
+    __shared__ uint32_t wmax[kThreads / 64];
+    const int tid = threadIdx.x % TPR, part = threadIdx.x / TPR;
+    const int64_t row = (int64_t)blockIdx.x * (kThreads / TPR) + part;
+    const bool here = row < rows;
+    const AT* const ar = a + (here ? row : rows - 1) * k;
+    const int pieces = k >> 3, turns = (pieces + TPR - 1) / TPR;
+    LhsPiece<AT> held[kHeld];
+    uint32_t top = 0;
+    if (turns <= kHeld) {
+#pragma unroll
+        for (int i = 0; i < kHeld; i++)
+            if (i < turns) held[i] = load_piece(ar + 8 * min(tid + i * TPR, pieces - 1));
+#pragma unroll
+        for (int i = 0; i < kHeld; i++)
+            if (i < turns) top = largest_bits(top, held[i]);
+    } else {
+        for (int pc = tid; pc < pieces; pc += TPR) top = largest_bits(top, load_piece(ar + 8 * pc));
+    }
+    float mx = largest_of<AT>(top);
+    if (any_not_finite(mx)) {
+        mx = 0.0f;
+        for (int pc = tid; pc < pieces; pc += TPR) mx = largest_finite(mx, load_piece(ar + 8 * pc));
+    }
+    uint32_t most = wave_max_nonneg_bits(mx);
+    if constexpr (TPR > 64) {
+        if ((threadIdx.x & 63) == 0) wmax[threadIdx.x >> 6] = most;
+        __syncthreads();
+        most = 0;
+#pragma unroll
+        for (int i = 0; i < TPR / 64; i++) most = max(most, wmax[part * (TPR / 64) + i]);
+    }
+    if (!here) return;
+    float inverse;
+    const float s = row_scale(most, with_sums ? kRowTopWithSums : kRowTop, inverse);
+    if (tid == 0) inv[row] = inverse;
+    uint8_t* const to = a16 + row * units * (512 * kPer);
+    auto emit = [&](int pc, const LhsPiece<AT>& x) __attribute__((always_inline)) {
+        float v[8];
+        unpack_piece(x, v);
+        // columns 8 pc ..: block blk of 32, half g, step 2 blk + a: piece 2 (step % 4) + g of chunk step / 4
+        const int blk = pc >> 2, at_g = (pc >> 1) & 1, step = 2 * blk + (pc & 1);
+        uint8_t* const at = to + (step >> 2) * (128 * kPer) + (2 * (step & 3) + at_g) * 16;
+        constexpr int perm[8] = {0, 2, 1, 3, 4, 6, 5, 7};
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] *= s;
+        HalfPack hi;
+#pragma unroll
+        for (int i = 0; i < 4; i++) hi.u[i] = narrow2(v[perm[2 * i]], v[perm[2 * i + 1]]);
+        *(half8*)at = hi.h;
+        if constexpr (kF32) {
+            HalfPack lo;
+            float rest[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float h = (float)hi.h[i];
+                rest[i] = fabsf(h) <= 65504.0f ? v[perm[i]] - h : 0.0f;  // (an infinity has no residual: inf - inf)
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) lo.u[i] = narrow2(rest[2 * i], rest[2 * i + 1]);
+            *(half8*)(at + 128) = lo.h;
+        }
+        if (with_sums) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) sum += v[i] + v[i + 1];
+            sum += dpp_move<0xB1>(sum);
+            sum += dpp_move<0x4E>(sum);  // the four threads of a block of 32
+            if ((pc & 3) == 0) {
+                const float sh = h2f(f2h(sum));
+                _Float16* const sp = (_Float16*)(sums + (row * units + (blk >> 3)) * 32) + (blk & 7);
+                sp[0] = (_Float16)sh;
+                sp[8] = (_Float16)(sum - sh);
+            }
+        }
+    };
+    if (turns <= kHeld) {
+#pragma unroll
+        for (int i = 0; i < kHeld; i++)
+            if (tid + i * TPR < pieces) emit(tid + i * TPR, held[i]);
+    } else {
+        for (int pc = tid; pc < pieces; pc += TPR) emit(pc, load_piece(ar + 8 * pc));
+    }
+}
+
+// Q4_0: Q8_0 codes as fp16 (exact), block scales in the place of the sums; what a unit has beyond the row is zeros.  Four neighbouring threads hold a block.
+template <typename AT>
+__global__ __launch_bounds__(256) void experts_prep_q8_kernel(const AT* __restrict__ a, int64_t rows, int k, int units, uint8_t* __restrict__ a16, uint8_t* __restrict__ sums, float* __restrict__ inv) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / (units * 32);
+    if (row >= rows) return;  // (whole blocks: a multiple of four threads)
+    const int pc = (int)(i - row * (units * 32)), pieces = k >> 3;
+    if (pc == 0) inv[row] = 1.0f;
+    const int blk = pc >> 2, sub = pc & 3, g = sub & 1, step = 2 * blk + (sub >> 1);  // columns 32 blk + 16 a + 8 g: step 2 blk + a
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (pc < pieces) unpack_piece(load_piece(a + row * k + pc * 8), v);
+    float mx = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(v[j]));
+    mx = fmaxf(mx, dpp_move<0xB1>(mx));
+    mx = fmaxf(mx, dpp_move<0x4E>(mx));
+    uint16_t dh;
+    const float id = q8_0_block_rule(mx, dh);
+    constexpr int perm[8] = {0, 2, 1, 3, 4, 6, 5, 7};
+    gd_u4 o;
+#pragma unroll
+    for (int j = 0; j < 4; j++) o[j] = pack_half2((float)q8_0_code(v[perm[2 * j]], id), (float)q8_0_code(v[perm[2 * j + 1]], id));
+    *(gd_u4*)(a16 + row * units * 512 + (step >> 2) * 128 + (2 * (step & 3) + g) * 16) = o;
+    if (sub == 0) {
+        uint16_t* const sp = (uint16_t*)(sums + (row * units + (blk >> 3)) * 32) + (blk & 7);
+        sp[0] = dh;
+        sp[8] = 0;
+    }
+}
+
+struct EgSpace {
+    int64_t sums, inv, bytes;  // (a16 first)
+};
+EgSpace eg_space(const ExpertCall& c) {
+    auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
+    const int64_t units = (c.k + 255) / 256;
+    EgSpace s;
+    s.sums = up(c.lhs_rows * units * 512 * (c.lhs_dtype == QMM_F32 && c.encoding != QMM_Q4_0 ? 2 : 1));
+    s.inv = s.sums + up(c.encoding == QMM_Q6_K ? 0 : c.lhs_rows * units * 32);
+    s.bytes = s.inv + up(c.lhs_rows * 4);
+    return s;
+}
+
+template <typename AT>
+hipError_t run_prep(const ExpertCall& c, const EgArgs& p, hipStream_t s) {
+    const AT* const a = (const AT*)c.lhs;
+    uint8_t *const a16 = (uint8_t*)p.a16, *const sums = (uint8_t*)p.sums;
+    float* const inv = (float*)p.inv;
+    const int k = (int)c.k;
+    if (c.encoding == QMM_Q4_0) {
+        experts_prep_q8_kernel<AT><<<dim3((unsigned)((c.lhs_rows * p.units * 32 + 255) / 256)), dim3(256), 0, s>>>(a, c.lhs_rows, k, p.units, a16, sums, inv);
+    } else {
+        const int with_sums = c.encoding != QMM_Q6_K;
+        if (k <= 1024) experts_prep_kernel<AT, 64><<<dim3((unsigned)((c.lhs_rows + 3) / 4)), dim3(256), 0, s>>>(a, c.lhs_rows, k, p.units, with_sums, a16, sums, inv);
+        else if (k <= 8192) experts_prep_kernel<AT, 256><<<dim3((unsigned)c.lhs_rows), dim3(256), 0, s>>>(a, c.lhs_rows, k, p.units, with_sums, a16, sums, inv);
+        else experts_prep_kernel<AT, 1024><<<dim3((unsigned)c.lhs_rows), dim3(1024), 0, s>>>(a, c.lhs_rows, k, p.units, with_sums, a16, sums, inv);
+    }
+    return hipGetLastError();
+}
+
+template <int ENC, int FM, bool HILO, bool GATED>
+hipError_t run_gemm(const EgArgs& p, const Routing& r, hipStream_t s) {
+    constexpr int lds = std::max(EgLds<ENC, FM, HILO>::kBytes, std::max(EgLds<ENC, 1, HILO>::kBytes, EgLds<ENC, std::min(FM, 2), HILO>::kBytes));
+    const hipError_t e = allow_full_lds<experts_gemm_kernel<ENC, FM, HILO, GATED>>();
+    if (e != hipSuccess) return e;
+    const int cols = GATED ? 128 : 256;
+    experts_gemm_kernel<ENC, FM, HILO, GATED><<<dim3(8, (unsigned)most_groups(r.pairs, r.experts, 32 * FM), (unsigned)((p.n + 8 * cols - 1) / (8 * cols))), dim3(64 * kEgWaves), lds, s>>>(p, r);
+    return hipGetLastError();
+}
+template <int ENC, int FM, bool HILO>
+hipError_t run_gemm(const EgArgs& p, const Routing& r, hipStream_t s) {
+    return p.gated ? run_gemm<ENC, FM, HILO, true>(p, r, s) : run_gemm<ENC, FM, HILO, false>(p, r, s);
+}
+// rows of a group: 32 fm
+template <int ENC>
+hipError_t run_gemm(const EgArgs& p, const Routing& r, int fm, bool hilo, hipStream_t s) {
+    if constexpr (ENC != QMM_Q4_0) {
+        if (hilo) return fm == 1 ? run_gemm<ENC, 1, true>(p, r, s) : run_gemm<ENC, 2, true>(p, r, s);
+        if (fm == 4) return run_gemm<ENC, 4, false>(p, r, s);
+    }
+    return fm == 1 ? run_gemm<ENC, 1, false>(p, r, s) : run_gemm<ENC, 2, false>(p, r, s);
+}
+
+// Rows of a group, in 32s: as many as an expert has on average, up to what the registers hold.
+int eg_rows(const ExpertCall& c, const Routing& r) {
+    const int64_t mean = r.pairs / r.experts;
+    const int most = c.encoding == QMM_Q4_0 || c.lhs_dtype == QMM_F32 ? 2 : 4;
+    return std::min(mean <= 32 ? 1 : mean <= 64 ? 2 : 4, most);
+}
+
+}  // namespace
+
+bool experts_gemm_supported(const ExpertCall& c, const Routing& r) {
+    if (kernel_disabled("experts_gemm")) return false;
+    const int64_t bpb = c.encoding == QMM_Q4_0 ? Q4_0_BPB : c.encoding == QMM_Q4_K ? Q4_K_BPB : c.encoding == QMM_Q5_K ? Q5_K_BPB : Q6_K_BPB, epb = c.encoding == QMM_Q4_0 ? 32 : 256;
+    const int64_t blocks = c.n * (c.k / epb);
+    if (blocks * bpb > 0x7fffffff || most_groups(r.pairs, r.experts, 64) > 65535) return false;  // (offsets in a matrix have 32 bits)
+    const uintptr_t all = (uintptr_t)c.w[0] | (uintptr_t)c.expert_stride[0] | (c.gated ? (uintptr_t)c.w[1] | (uintptr_t)c.expert_stride[1] : 0);
+    if (c.encoding == QMM_Q4_0) return (all & 1) == 0;
+    if (all & 3) return false;
+    return c.encoding != QMM_Q6_K || blocks % 2 == 0;  // (an odd last block would be read two bytes beyond its end)
+}
+
+int64_t experts_gemm_workspace_bytes(const ExpertCall& c) { return eg_space(c).bytes; }
+
+hipError_t launch_experts_gemm(const ExpertCall& c, const Routing& r, void* out, bool out_bf16, void* workspace, hipStream_t s) {
+    const EgSpace space = eg_space(c);
+    const uint8_t* const ws = (const uint8_t*)workspace;
+    const EgArgs p{ws,      ws + space.sums, (const float*)(ws + space.inv), {c.w[0], c.w[1]}, {c.expert_stride[0], c.expert_stride[1]}, c.lhs_top, (int)c.n, (int)c.k, (int)((c.k + 255) / 256),
+                   c.gated, out,             out_bf16};
+    const hipError_t e = c.lhs_dtype == QMM_F32 ? run_prep<float>(c, p, s) : run_prep<uint16_t>(c, p, s);
+    if (e != hipSuccess) return e;
+    const bool hilo = c.lhs_dtype == QMM_F32;
+    const int fm = eg_rows(c, r);
+    switch (c.encoding) {
+        case QMM_Q4_0: return run_gemm<QMM_Q4_0>(p, r, fm, hilo, s);
+        case QMM_Q4_K: return run_gemm<QMM_Q4_K>(p, r, fm, hilo, s);
+        case QMM_Q5_K: return run_gemm<QMM_Q5_K>(p, r, fm, hilo, s);
+        default: return run_gemm<QMM_Q6_K>(p, r, fm, hilo, s);
+    }
+}
+
+}  // namespace qmm

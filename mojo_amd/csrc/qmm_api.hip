@@ -1312,7 +1312,7 @@ int qmm_group_experts(const int32_t* ids, int64_t pairs, int experts, int32_t* o
 }
 
 // The products' own share of the workspace, then (a sum) the results of the pairs.
-static int64_t experts_product_bytes(const qmm::ExpertCall& c) { return up256(qmm::experts_rows_workspace_bytes(c)); }
+static int64_t experts_product_bytes(const qmm::ExpertCall& c) { return up256(std::max(qmm::experts_rows_workspace_bytes(c), qmm::experts_gemm_workspace_bytes(c))); }
 
 int64_t qmm_matmul_experts_workspace_bytes(int op, int encoding, int lhs_dtype, int64_t lhs_rows, int64_t tokens, int top, int experts, int64_t n, int64_t k, int flags) {
     int64_t epb, bpb;
@@ -1355,7 +1355,9 @@ int qmm_matmul_experts(int op, int encoding, const qmm_routing* routing, const v
     if (need > 0 && !aligned(workspace, 256)) return fail(QMM_ERR_INVALID, "qmm_matmul_experts: workspace must be 256-byte aligned");
     const bool out_bf16 = flags & QMM_FLAG_OUT_BF16;
     float* const y = sum ? (float*)((char*)workspace + experts_product_bytes(c)) : nullptr;
-    if (int rc = hip_status(qmm::launch_experts_rows(c, r, sum ? (void*)y : out, out_bf16 && !sum, workspace, (hipStream_t)stream), "qmm_matmul_experts")) return rc;
+    const hipError_t e = qmm::experts_gemm_supported(c, r) ? qmm::launch_experts_gemm(c, r, sum ? (void*)y : out, out_bf16 && !sum, workspace, (hipStream_t)stream)
+                                                          : qmm::launch_experts_rows(c, r, sum ? (void*)y : out, out_bf16 && !sum, workspace, (hipStream_t)stream);
+    if (int rc = hip_status(e, "qmm_matmul_experts")) return rc;
     if (!sum) return QMM_OK;
     return hip_status(qmm::launch_experts_combine(r, y, n, residual, residual_dtype, out, out_bf16, (hipStream_t)stream), "qmm_matmul_experts(sum)");
 }

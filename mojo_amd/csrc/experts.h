@@ -76,6 +76,11 @@ hipError_t launch_experts_rows(const ExpertCall& c, const Routing& r, void* out,
 bool experts_gemm_supported(const ExpertCall& c, const Routing& r);
 int64_t experts_gemm_workspace_bytes(const ExpertCall& c);
 hipError_t launch_experts_gemm(const ExpertCall& c, const Routing& r, void* out, bool out_bf16, void* workspace, hipStream_t s);
+// experts_small.hip: a few rows for each expert; the sum: one token
+bool experts_small_wanted(const ExpertCall& c, const Routing& r);
+hipError_t launch_experts_small(const ExpertCall& c, const Routing& r, void* out, bool out_bf16, hipStream_t s);
+bool experts_sum_small_wanted(const ExpertCall& c, const Routing& r);
+hipError_t launch_experts_sum_small(const ExpertCall& c, const Routing& r, const void* residual, int residual_dtype, void* out, bool out_bf16, hipStream_t s);
 // out[t] = residual[t] + sum over j of weights[top t + j] y[top t + j], in that order (pairs without an expert left out); residual: null, fp32 or bf16
 hipError_t launch_experts_combine(const Routing& r, const float* y, int64_t n, const void* residual, int residual_dtype, void* out, bool out_bf16, hipStream_t s);
 

@@ -18,7 +18,7 @@ namespace qmm {
 namespace {
 
 constexpr int kRouteThreads = 1024, kRouteWaves = kRouteThreads / 64;
-constexpr int kRouteBlocks = 256;  // workgroups at most: each adds up the counts of those before it
+constexpr int kRouteBlocks = 512;  // workgroups at most: each adds up the counts of those before it
 
 template <int CTRL>
 __device__ __forceinline__ uint64_t dpp_move64(uint64_t v) {
@@ -258,14 +258,24 @@ __global__ __launch_bounds__(kRouteThreads) void place_kernel(const int32_t* __r
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), runs = experts + 1;
     int* const start = route_lds + kRouteWaves * runs;
     int* const before = start + runs;
-    for (int e = threadIdx.x; e < runs; e += kRouteThreads) {
+    for (int e = threadIdx.x; e < runs; e += kRouteThreads) start[e] = before[e] = 0;
+    __syncthreads();
+    // the counts of all workgroups and of those before this one: as many threads share an expert's as there are, each eight loads at a time
+    const int width = (runs + 63) / 64 * 64, shares = max(1, kRouteThreads / width), blocks_all = (int)gridDim.x;
+    for (int e = (int)threadIdx.x % width; e < runs && (int)threadIdx.x < shares * width; e += kRouteThreads) {
         int sum = 0, mine = 0;
-        for (int b = 0; b < (int)gridDim.x; b++) {
-            if (b == (int)blockIdx.x) mine = sum;
-            sum += blocks[(int64_t)b * runs + e];
+        for (int b0 = (int)threadIdx.x / width; b0 < blocks_all; b0 += 8 * shares) {
+            int v[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = b0 + i * shares < blocks_all ? blocks[(int64_t)(b0 + i * shares) * runs + e] : 0;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                sum += v[i];
+                mine += b0 + i * shares < (int)blockIdx.x ? v[i] : 0;
+            }
         }
-        start[e] = sum;
-        before[e] = mine;
+        atomicAdd(start + e, sum);
+        atomicAdd(before + e, mine);
     }
     exclusive_sums(start, runs, wave, lane);
     if (blockIdx.x == 0)
@@ -277,10 +287,10 @@ __global__ __launch_bounds__(kRouteThreads) void place_kernel(const int32_t* __r
     place_pairs(ids, from, min(from + per, pairs), experts, route_lds, start, order, wave, lane);
 }
 
-// Tokens (pairs, with top 1) of a workgroup: all, up to 1024 pairs; else two a wavefront and as many more as leave kRouteBlocks workgroups.
+// Tokens (pairs, with top 1) of a workgroup: all, up to 1024 pairs; else one a wavefront and as many more as leave kRouteBlocks workgroups.
 int64_t route_per(int64_t tokens, int top) {
     if (tokens * top <= kRouteThreads) return tokens;
-    const int64_t least = top == 1 ? kRouteThreads : 2 * kRouteWaves;
+    const int64_t least = top == 1 ? kRouteThreads : kRouteWaves;
     return std::max(least, (tokens + kRouteBlocks - 1) / kRouteBlocks);
 }
 size_t sort_lds(int experts) { return (size_t)(kRouteWaves + 2) * (experts + 1) * 4; }

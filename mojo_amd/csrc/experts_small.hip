@@ -1,0 +1,141 @@
+// The experts' products with a few rows for each expert: the kernel for a few lhs rows (small_body.h), a workgroup's rows being some of an expert's pairs and its weights that expert's.  One launch, no workspace.
+//
+// Groups of up to MROWS pairs are counted over the experts (blockIdx.y; as many as there can be, those beyond the last leave at once), the tiles of 16 weight rows of each over blockIdx.x.  With one token
+// every pair is a group and nothing is looked up.  What bounds it is the way to the first product and then the weights, as in the kernel that it is made of.
+//
+// The weighted sum of a token whose experts all have rows of their own is a product too: the experts' super-blocks one after the other as one long K, each times its expert's weight, so that one launch ends
+// with the token's results (a second launch, for the sum, is 2.5 us and the pairs' results written and read).
+#include <math.h>
+
+#include <algorithm>
+
+#include "small_body.h"
+
+namespace qmm {
+
+namespace {
+
+template <int ENC, int MROWS, typename AT, int MODE, int EX>
+__global__ __launch_bounds__(64 * kSmallWaves) void experts_small_kernel(MmMats mats, const AT* __restrict__ a, int m, int k, SmallCut cut, SmallExperts ex) {
+    small_body<ENC, MROWS, AT, MODE, EX>(mats, a, m, k, cut, ex);
+}
+
+struct EsPlan {
+    int waves, groups, per, grid, chunk;
+    size_t lds;
+};
+// tiles: of one group of rows; groups_y: groups of rows; nblk: super-blocks that a workgroup walks
+EsPlan es_plan(int encoding, int mrows, int64_t tiles, int64_t groups_y, int64_t nblk) {
+    EsPlan p;
+    p.groups = (int)((nblk + kSmallWaves - 1) / kSmallWaves);
+    p.waves = (int)((nblk + p.groups - 1) / p.groups);
+    const int per_cu = std::max(1, kSmallWaves / p.waves);
+    const int64_t places = std::max<int64_t>(1, (int64_t)compute_units() * per_cu / groups_y);
+    p.per = (int)((tiles + places - 1) / places);
+    p.grid = (int)((tiles + p.per - 1) / p.per);
+    const int slot = encoding == QMM_Q4_0 || encoding == QMM_Q4_K ? SmallItem<QMM_Q4_K>::kSlot : encoding == QMM_Q5_K ? SmallItem<QMM_Q5_K>::kSlot : SmallItem<QMM_Q6_K>::kSlot;
+    const int lr = mrows <= 4 ? 1 : mrows / 4, ring = p.waves * 2 * slot, bytes = (p.waves + (p.groups > 1 ? 1 : 0)) * lr * 256;
+    p.chunk = std::min(std::min(p.per, 254), (kLdsPerCu / per_cu - ring) / bytes);
+    p.lds = (size_t)ring + (size_t)p.chunk * bytes;
+    return p;
+}
+
+template <int ENC, int MROWS, typename AT, int MODE, int EX>
+hipError_t run_small(const ExpertCall& c, const SmallExperts& ex, int64_t groups_y, int64_t expected, void* out, bool out_bf16, hipStream_t s) {
+    const int tile = MODE == kSmallGated ? 8 : 16;
+    const EsPlan p = es_plan(ENC, MROWS, (c.n + tile - 1) / tile, expected, c.k / 256 * (EX == kSmallOverExperts ? ex.r.top : 1));
+    const hipError_t e = allow_full_lds<experts_small_kernel<ENC, MROWS, AT, MODE, EX>>();
+    if (e != hipSuccess) return e;
+    MmMats mats{};
+    for (int j = 0; j < kLanesMaxMats; j++) {
+        mats.w[j] = c.w[j == 1 && c.gated ? 1 : 0];
+        mats.out[j] = (float*)out;
+        mats.n[j] = (int)c.n;
+    }
+    mats.count = 1;
+    const SmallCut cut{p.per, p.grid, (uint32_t)p.waves | (uint32_t)p.chunk << 8 | (uint32_t)out_bf16 << 16 | (uint32_t)p.groups << 18};
+    experts_small_kernel<ENC, MROWS, AT, MODE, EX><<<dim3((unsigned)p.grid, (unsigned)groups_y), dim3((unsigned)(64 * p.waves)), p.lds, s>>>(mats, (const AT*)c.lhs, MROWS, (int)c.k, cut, ex);
+    return hipGetLastError();
+}
+template <int ENC, int MROWS, typename AT>
+hipError_t run_small(const ExpertCall& c, const SmallExperts& ex, int64_t groups_y, int64_t expected, void* out, bool out_bf16, hipStream_t s) {
+    return c.gated ? run_small<ENC, MROWS, AT, kSmallGated, kSmallByExpert>(c, ex, groups_y, expected, out, out_bf16, s)
+                   : run_small<ENC, MROWS, AT, kSmallPlain, kSmallByExpert>(c, ex, groups_y, expected, out, out_bf16, s);
+}
+
+// Rows of a group: what an expert that has any gets, on average over those (each token's experts are others).
+int es_rows(const ExpertCall& c, const Routing& r, int64_t& expected) {
+    const int64_t tokens = r.pairs / r.top, most = small_most_rows(c.lhs_dtype);
+    if (tokens == 1) {
+        expected = r.pairs;
+        return 1;
+    }
+    const double with = r.experts * (1.0 - pow(1.0 - (double)r.top / r.experts, (double)tokens)), mean = r.pairs / std::max(with, 1.0);
+    const int rows = tokens <= 4 || mean <= 2.5 ? 4 : mean <= 5.5 || most == 8 ? 8 : 16;
+    expected = std::max<int64_t>(1, (int64_t)(with * std::max(1.0, mean / rows)));
+    return rows;
+}
+int64_t es_groups(const Routing& r, int rows) { return r.pairs == r.top ? r.pairs : most_groups(r.pairs, r.experts, rows); }
+
+template <int ENC>
+hipError_t run_small(const ExpertCall& c, const SmallExperts& ex, void* out, bool out_bf16, hipStream_t s) {
+    int64_t expected;
+    const int rows = es_rows(c, ex.r, expected);
+    const int64_t groups = es_groups(ex.r, rows);
+    if (c.lhs_dtype == QMM_F32)
+        return rows == 1   ? run_small<ENC, 1, float>(c, ex, groups, expected, out, out_bf16, s)
+               : rows == 4 ? run_small<ENC, 4, float>(c, ex, groups, expected, out, out_bf16, s)
+                           : run_small<ENC, 8, float>(c, ex, groups, expected, out, out_bf16, s);
+    return rows == 1   ? run_small<ENC, 1, uint16_t>(c, ex, groups, expected, out, out_bf16, s)
+           : rows == 4 ? run_small<ENC, 4, uint16_t>(c, ex, groups, expected, out, out_bf16, s)
+           : rows == 8 ? run_small<ENC, 8, uint16_t>(c, ex, groups, expected, out, out_bf16, s)
+                       : run_small<ENC, 16, uint16_t>(c, ex, groups, expected, out, out_bf16, s);
+}
+template <int ENC>
+hipError_t run_sum(const ExpertCall& c, const SmallExperts& ex, void* out, bool out_bf16, hipStream_t s) {
+    const int64_t tokens = ex.r.pairs / ex.r.top;
+    return c.lhs_dtype == QMM_F32 ? run_small<ENC, 1, float, kSmallPlain, kSmallOverExperts>(c, ex, tokens, tokens, out, out_bf16, s)
+                                  : run_small<ENC, 1, uint16_t, kSmallPlain, kSmallOverExperts>(c, ex, tokens, tokens, out, out_bf16, s);
+}
+
+bool es_takes(const ExpertCall& c) {
+    if (kernel_disabled("experts_small")) return false;
+    if (c.k % 256 || c.k > (1 << 20)) return false;
+    const uintptr_t all = (uintptr_t)c.w[0] | (uintptr_t)c.expert_stride[0] | (c.gated ? (uintptr_t)c.w[1] | (uintptr_t)c.expert_stride[1] : 0);
+    if (c.encoding == QMM_Q4_K || c.encoding == QMM_Q5_K) return (all & 15) == 0;
+    if (all & 3) return false;
+    return c.encoding == QMM_Q4_0 || c.n * (c.k / 256) % 2 == 0;  // (loads of four bytes at least: the last block of a matrix has to end at a multiple of four)
+}
+
+}  // namespace
+
+bool experts_small_wanted(const ExpertCall& c, const Routing& r) {
+    if (!es_takes(c)) return false;
+    int64_t expected;
+    const int rows = es_rows(c, r, expected);
+    return r.pairs <= 4096 && es_groups(r, rows) <= 65535 && r.pairs <= (int64_t)r.experts * small_most_rows(c.lhs_dtype);
+}
+
+hipError_t launch_experts_small(const ExpertCall& c, const Routing& r, void* out, bool out_bf16, hipStream_t s) {
+    const SmallExperts ex{r, {c.expert_stride[0], c.expert_stride[1]}, c.lhs_top, nullptr, 0};
+    switch (c.encoding) {
+        case QMM_Q4_0: return run_small<QMM_Q4_0>(c, ex, out, out_bf16, s);
+        case QMM_Q4_K: return run_small<QMM_Q4_K>(c, ex, out, out_bf16, s);
+        case QMM_Q5_K: return run_small<QMM_Q5_K>(c, ex, out, out_bf16, s);
+        default: return run_small<QMM_Q6_K>(c, ex, out, out_bf16, s);
+    }
+}
+
+bool experts_sum_small_wanted(const ExpertCall& c, const Routing& r) { return es_takes(c) && r.pairs == r.top && c.k / 256 * r.top / kSmallWaves < 0x1fff; }
+
+hipError_t launch_experts_sum_small(const ExpertCall& c, const Routing& r, const void* residual, int residual_dtype, void* out, bool out_bf16, hipStream_t s) {
+    const SmallExperts ex{r, {c.expert_stride[0], c.expert_stride[1]}, c.lhs_top, residual, residual_dtype == QMM_BF16};
+    switch (c.encoding) {
+        case QMM_Q4_0: return run_sum<QMM_Q4_0>(c, ex, out, out_bf16, s);
+        case QMM_Q4_K: return run_sum<QMM_Q4_K>(c, ex, out, out_bf16, s);
+        case QMM_Q5_K: return run_sum<QMM_Q5_K>(c, ex, out, out_bf16, s);
+        default: return run_sum<QMM_Q6_K>(c, ex, out, out_bf16, s);
+    }
+}
+
+}  // namespace qmm

@@ -4,6 +4,8 @@
 //
 // The elements equal to the running maximum are counted (c) and kept out of the sum (s), so that S = c + s and log S = log1p(c - 1 + s): a row whose
 // largest value holds all but 1e-6 of the mass has a log probability of 1e-6, not of what fp32 leaves of 1 + 1e-6.  c is a number, so counting it takes no rounding either.
+// An element costs one multiply-add, one exponential (four times an ordinary instruction), a sum, a multiply-add for t and a clamp that makes 0 x -inf a 0: exp(x - m) is 2^(x L - f) with L = log2 e and
+// f = m L rounded; what that rounding moved, the same for every element, is put right where the wavefronts are joined.
 // Parts of a row (lanes, wavefronts, workgroups) each have their (m, c, s, t) and are joined with exp(m_i - m).
 //
 // Alternatives.  A value that is among the `top` largest lies in one of the `top` runs of neighbouring values (four lanes' loads: 16 fp32 or 32 bf16 values) with the largest maxima, equal ones by
@@ -41,57 +43,68 @@ __device__ __forceinline__ uint32_t order_of(float x) {
 __device__ __forceinline__ uint64_t key_of(float x, uint32_t index) { return (uint64_t)order_of(x) << 32 | (uint32_t)~index; }
 __device__ __forceinline__ uint32_t index_of(uint64_t key) { return ~(uint32_t)key; }
 
-// exp(d), d <= 0
-__device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * 1.44269504088896f); }
+constexpr float kLog2e = 1.44269504088896f, kLn2 = 0.693147180559945f;
+__device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }  // d <= 0
 // what stands for -inf where it meets a factor of exp(-inf) = 0
 constexpr float kLpFloor = -150.0f;
+// Beyond, the next fp32 number is 128 lower and its exponential 0, as that of all others (f = inf); up to here the rounding of m L is no more than 64, and 2 to that power a number.
+constexpr float kLpFar = 1073741824.0f;
 
 // b joins a.  (m = -inf: nothing but -inf so far, whose number does not matter.)
 __device__ __forceinline__ void join(LpState& a, const LpState& b) {
-    const bool more = b.m > a.m;
-    const LpState hi = more ? b : a, lo = more ? a : b;
-    a = hi;
-    if (lo.m == hi.m) {
-        a.c += lo.c;
-        a.s += lo.s;
-        a.t += lo.t;
-    } else {
-        const float d = fmaxf(lo.m - hi.m, kLpFloor), f = exp_of(d), n = (float)lo.c + lo.s;
-        a.s = fmaf(f, n, a.s);
-        a.t = fmaf(f, fmaf(d, n, lo.t), a.t);
-    }
-}
-__device__ __forceinline__ LpState from_lane(const LpState& a, int mask) {
-    return {__shfl_xor(a.m, mask), __shfl_xor(a.s, mask), __shfl_xor(a.t, mask), __shfl_xor(a.c, mask)};
-}
-__device__ __forceinline__ void wave_join(LpState& a) {
-#pragma unroll
-    for (int mask = 32; mask; mask >>= 1) {
-        const LpState b = from_lane(a, mask);
-        join(a, b);
-    }
+    const bool more = b.m > a.m, even = b.m == a.m;
+    const float lm = more ? a.m : b.m, ls = more ? a.s : b.s, lt = more ? a.t : b.t, hs = more ? b.s : a.s, ht = more ? b.t : a.t;
+    const int lc = more ? a.c : b.c, hc = more ? b.c : a.c;
+    a.m = more ? b.m : a.m;
+    const float d = fmaxf(lm - a.m, kLpFloor), f = exp_of(d), n = (float)lc + ls;
+    a.c = even ? hc + lc : hc;
+    a.s = even ? hs + ls : fmaf(f, n, hs);
+    a.t = even ? ht + lt : fmaf(f, fmaf(d, n, lt), ht);
 }
 
-__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int mask) {
-    return (uint64_t)(uint32_t)__shfl_xor((int)(v >> 32), mask) << 32 | (uint32_t)__shfl_xor((int)v, mask);
+// The value of lane ^ MASK, without LDS: DPP within 16 lanes (4: mirrored in eight, then in four), exchanges of rows beyond.
+template <int MASK>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t v, int lane) {
+    if constexpr (MASK == 1) return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xf, 0xf, true);
+    if constexpr (MASK == 2) return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xf, 0xf, true);
+    if constexpr (MASK == 4) return (uint32_t)__builtin_amdgcn_mov_dpp(__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xf, 0xf, true), 0x1B, 0xf, 0xf, true);
+    if constexpr (MASK == 8) return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x128, 0xf, 0xf, true);
+    if constexpr (MASK == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        return (lane & 16) ? r[0] : r[1];
+    }
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return (lane & 32) ? r[0] : r[1];
 }
-// One step of a bitonic sort over the lanes: the larger of a pair to the lane with (lane & mask) == 0, if `falling`.
-__device__ __forceinline__ void exchange(uint64_t& v, int lane, int mask, bool falling) {
-    const uint64_t o = shfl_xor64(v, mask);
-    const bool low = (lane & mask) == 0;
-    v = (v > o) == (low == falling) ? v : o;
+template <int MASK>
+__device__ __forceinline__ float lane_xor(float v, int lane) { return __uint_as_float(lane_xor<MASK>(__float_as_uint(v), lane)); }
+template <int MASK = 32>
+__device__ __forceinline__ void wave_join(LpState& a, int lane) {
+    const LpState b{lane_xor<MASK>(a.m, lane), lane_xor<MASK>(a.s, lane), lane_xor<MASK>(a.t, lane), (int)lane_xor<MASK>((uint32_t)a.c, lane)};
+    join(a, b);
+    if constexpr (MASK > 1) wave_join<MASK / 2>(a, lane);
 }
+
+// One step of a bitonic sort over the lanes: the larger of a pair to the lane that wants it.
+template <int MASK>
+__device__ __forceinline__ void exchange(uint64_t& v, int lane, bool larger) {
+    const uint64_t o = (uint64_t)lane_xor<MASK>((uint32_t)(v >> 32), lane) << 32 | lane_xor<MASK>((uint32_t)v, lane);
+    v = (v > o) == larger ? v : o;
+}
+template <int SIZE, int MASK>
+__device__ __forceinline__ void merge_step(uint64_t& v, int lane) {
+    exchange<MASK>(v, lane, ((lane & MASK) == 0) == (SIZE == 64 || (lane & SIZE) == 0));
+    if constexpr (MASK > 1) merge_step<SIZE, MASK / 2>(v, lane);
+}
+template <int SIZE = 2>
 __device__ __forceinline__ void sort64(uint64_t& v, int lane) {  // falling
-#pragma unroll
-    for (int size = 2; size <= 64; size *= 2)
-#pragma unroll
-        for (int mask = size / 2; mask; mask >>= 1) exchange(v, lane, mask, size == 64 || (lane & size) == 0);
+    merge_step<SIZE, SIZE / 2>(v, lane);
+    if constexpr (SIZE < 64) sort64<SIZE * 2>(v, lane);
 }
 // a: falling; reversed: another falling list, last entry first.  The 64 largest of both, falling.
 __device__ __forceinline__ void merge64(uint64_t& a, uint64_t reversed, int lane) {
     a = a > reversed ? a : reversed;
-#pragma unroll
-    for (int mask = 32; mask; mask >>= 1) exchange(a, lane, mask, true);
+    merge_step<64, 32>(a, lane);
 }
 
 // The lists of the workgroup's wavefronts (falling, one entry a lane) to one, in lists[0 .. 63] (visible to all afterwards).
@@ -128,6 +141,13 @@ __device__ __forceinline__ void top_keys(int count, int top, uint64_t* lists, in
     merge_waves<WAVES>(mine, lists, wave, lane);
 }
 
+// The largest of three (no NaN among the results unless all are); the compiler's own would first make each value a quiet one.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
 // A row as 16-byte loads at multiples of 16 bytes: load v holds the values v * kPer - skew .. of the row; the first and the last one may hold fewer.
 template <typename T>
 struct LpRow {
@@ -140,26 +160,25 @@ struct LpRow {
     }
     __device__ __forceinline__ int loads() const { return (skew + vocab + kPer - 1) / kPer; }
     __device__ __forceinline__ bool whole(int v) const { return v * kPer >= skew && (v + 1) * kPer - skew <= vocab; }
-    // the values of load v; -inf for those that the row does not have
-    __device__ __forceinline__ void get(int v, float (&x)[kPer]) const {
-        lp_u4 raw;
-        if (whole(v)) {
-            raw = *(const lp_u4*)(aligned + (int64_t)v * kPer);
-        } else {
-            T e[kPer];
-#pragma unroll
-            for (int i = 0; i < kPer; i++) {
-                const int at = v * kPer + i - skew;
-                if constexpr (sizeof(T) == 4) e[i] = at >= 0 && at < vocab ? aligned[(int64_t)v * kPer + i] : -__builtin_inff();
-                else e[i] = at >= 0 && at < vocab ? aligned[(int64_t)v * kPer + i] : (T)0xff80;
-            }
-            __builtin_memcpy(&raw, e, 16);
-        }
+    static __device__ __forceinline__ void unpack(const lp_u4& raw, float (&x)[kPer]) {
 #pragma unroll
         for (int i = 0; i < kPer; i++) {
             if constexpr (sizeof(T) == 4) x[i] = __uint_as_float(raw[i]);
             else x[i] = __uint_as_float((i & 1) ? raw[i >> 1] & 0xffff0000u : raw[i >> 1] << 16);
         }
+    }
+    // load v; -inf in the place of values that the row does not have
+    __device__ __forceinline__ lp_u4 edge(int v) const {
+        lp_u4 raw;
+        T e[kPer];
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            const int at = v * kPer + i - skew;
+            if constexpr (sizeof(T) == 4) e[i] = at >= 0 && at < vocab ? aligned[(int64_t)v * kPer + i] : -__builtin_inff();
+            else e[i] = at >= 0 && at < vocab ? aligned[(int64_t)v * kPer + i] : (T)0xff80;
+        }
+        __builtin_memcpy(&raw, e, 16);
+        return raw;
     }
     __device__ __forceinline__ float at(int64_t i) const { return load_f32(aligned, i + skew); }
 };
@@ -206,40 +225,39 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(const T* __restric
     const bool wanted = out.top > 0;
 
     const int whole0 = row.skew ? 1 : 0, whole1 = min(end, (row.skew + vocab) / kPer);  // loads that the row fills
-    float m = -__builtin_inff(), s = 0.0f, t = 0.0f;
-    int c = 0;  // (m and c: of the wavefront; s and t: of the lane)
-    for (int v0 = first + wave * 64 * kLpLoads; v0 < end; v0 += kLpStep) {
-        float x[kLpLoads][kPer], most[kLpLoads];
+    lp_u4 next[kLpLoads];
+    auto load = [&](int v0) __attribute__((always_inline)) {
         if (v0 >= whole0 && v0 + 64 * kLpLoads <= whole1) {
-            // (inside the row: all loads are asked for together)
-            lp_u4 raw[kLpLoads];
 #pragma unroll
-            for (int j = 0; j < kLpLoads; j++) raw[j] = *(const lp_u4*)(row.aligned + (int64_t)(v0 + j * 64 + lane) * kPer);
-#pragma unroll
-            for (int j = 0; j < kLpLoads; j++)
-#pragma unroll
-                for (int i = 0; i < kPer; i++) {
-                    if constexpr (sizeof(T) == 4) x[j][i] = __uint_as_float(raw[j][i]);
-                    else x[j][i] = __uint_as_float((i & 1) ? raw[j][i >> 1] & 0xffff0000u : raw[j][i >> 1] << 16);
-                }
+            for (int j = 0; j < kLpLoads; j++) next[j] = *(const lp_u4*)(row.aligned + (int64_t)(v0 + j * 64 + lane) * kPer);
         } else {
-#pragma unroll
+            constexpr uint32_t kNone = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
+#pragma unroll 1
             for (int j = 0; j < kLpLoads; j++) {
                 const int v = v0 + j * 64 + lane;
-                if (v < end) row.get(v, x[j]);
-                else
+                lp_u4 raw{kNone, kNone, kNone, kNone};
+                if (v < end) raw = row.whole(v) ? *(const lp_u4*)(row.aligned + (int64_t)v * kPer) : row.edge(v);
 #pragma unroll
-                    for (int i = 0; i < kPer; i++) x[j][i] = -__builtin_inff();
+                for (int i = 0; i < kLpLoads; i++) next[i] = i == j ? raw : next[i];
             }
         }
-        float all = -__builtin_inff();
+    };
+    float m = -__builtin_inff(), f = 0.0f, s = 0.0f, t = 0.0f;  // m and f = m L: of the wavefront; s and t (in units of log 2): of the lane
+    int c = 0;                                                  // of the wavefront
+    int v0 = first + wave * 64 * kLpLoads;
+    if (v0 < end) load(v0);
+    for (; v0 < end; v0 += kLpStep) {
+        float x[kLpLoads][kPer], most[kLpLoads], all = -__builtin_inff();
 #pragma unroll
         for (int j = 0; j < kLpLoads; j++) {
-            most[j] = x[j][0];
+            LpRow<T>::unpack(next[j], x[j]);
+            most[j] = x[j][kPer - 1];
 #pragma unroll
-            for (int i = 1; i < kPer; i++) most[j] = fmaxf(most[j], x[j][i]);
+            for (int i = 0; i + 1 < kPer - 1; i += 2) most[j] = max3(most[j], x[j][i], x[j][i + 1]);
+            if constexpr (kPer % 2 == 0) most[j] = fmaxf(most[j], x[j][kPer - 2]);
             all = fmaxf(all, most[j]);
         }
+        if (v0 + kLpStep < end) load(v0 + kLpStep);  // on its way meanwhile
         if (wanted) {
             // the maximum of a run, four lanes, is in all of them; lane j of four keeps that of load j
             float keep = 0.0f;
@@ -253,15 +271,24 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(const T* __restric
             if (run * 4 < end - first) runs[run] = keep;
         }
         if (__any(all >= m)) {
-            // a new maximum, or one equal to it: rare once some steps have passed
+            // a new maximum, or one equal to it
             float now = fmaxf(all, m);
-#pragma unroll
-            for (int mask = 32; mask; mask >>= 1) now = fmaxf(now, __shfl_xor(now, mask));
+            now = fmaxf(now, lane_xor<32>(now, lane));
+            now = fmaxf(now, lane_xor<16>(now, lane));
+            now = fmaxf(now, lane_xor<8>(now, lane));
+            now = fmaxf(now, lane_xor<4>(now, lane));
+            now = fmaxf(now, lane_xor<2>(now, lane));
+            now = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(fmaxf(now, lane_xor<1>(now, lane)))));
             if (now > m) {
-                const float d = fmaxf(m - now, kLpFloor), f = exp_of(d), n = lane == 0 ? (float)c : 0.0f;  // (what was the maximum is none now)
-                t = f * fmaf(d, s + n, t);
-                s = f * (s + n);
+                // (what was the maximum is none now: c elements of 2^(m L - f))
+                const float g = fabsf(now) > kLpFar ? __builtin_inff() : now * kLog2e;
+                if (m > -__builtin_inff() && f < __builtin_inff()) {
+                    const float d = fmaxf(f - g, 1.5f * kLpFloor), by = __builtin_amdgcn_exp2f(d), r = fmaf(m, kLog2e, -f), n = lane == 0 ? (float)c * __builtin_amdgcn_exp2f(r) : 0.0f;
+                    t = by * (fmaf(d, s, t) + (d + r) * n);
+                    s = by * (s + n);
+                }
                 m = now;
+                f = g;
                 c = 0;
             }
 #pragma unroll
@@ -270,30 +297,47 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(const T* __restric
                 for (int i = 0; i < kPer; i++) {
                     const bool is = x[j][i] == m;
                     c += (int)__popcll(__ballot(is));
-                    const float d = x[j][i] - m, e = is ? 0.0f : exp_of(d);
-                    s += e;
-                    t = fmaf(is ? 0.0f : fmaxf(d, kLpFloor), e, t);
-                }
-        } else {
-#pragma unroll
-            for (int j = 0; j < kLpLoads; j++)
-#pragma unroll
-                for (int i = 0; i < kPer; i++) {
-                    const float d = x[j][i] - m, e = exp_of(d);
-                    s += e;
-                    t = fmaf(fmaxf(d, kLpFloor), e, t);
+                    x[j][i] = is ? -__builtin_inff() : x[j][i];
                 }
         }
+        float s2[2] = {0.0f, 0.0f}, t2[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < kLpLoads; j++)
+#pragma unroll
+            for (int i = 0; i < kPer; i++) {
+                const float d = fmaf(x[j][i], kLog2e, -f), e = __builtin_amdgcn_exp2f(d);
+                s2[i & 1] += e;
+                t2[i & 1] = fmaf(fmaxf(d, 1.5f * kLpFloor), e, t2[i & 1]);
+            }
+        s += s2[0] + s2[1];
+        t += t2[0] + t2[1];
     }
-    LpState a{m, s, t, lane == 0 ? c : 0};
-    wave_join(a);
+    // f is m L but for its rounding r: every element was 2^r times what it is, with r more in its exponent
+    const float r = fabsf(m) <= kLpFar ? fmaf(m, kLog2e, -f) : 0.0f, by = __builtin_amdgcn_exp2f(-r);
+    LpState a{m, s * by, (t - r * s) * by * kLn2, lane == 0 ? c : 0};
+    wave_join(a, lane);
     if (lane == 0) waves[wave] = a;
     __syncthreads();
     a = waves[0];
 #pragma unroll
-    for (int w = 1; w < kLpWaves; w++) join(a, waves[w]);
+    for (int w = 1; w < kLpWaves; w++) {
+        const LpState b = waves[w];
+        join(a, b);
+    }
     if (wanted) {
         const int count = (end - first + 3) / 4;  // runs of this part
+        if (a.s != a.s) {
+            // There is a NaN.  (One that signals would have hidden its neighbours from the maxima above.)
+            for (int run = threadIdx.x; run < count; run += kLpThreads) {
+                float most = __builtin_nanf("");
+                for (int i = 0; i < kRun; i++) {
+                    const int64_t at = (first + (int64_t)run * 4) * kPer + i - row.skew;
+                    if (at >= 0 && at < vocab && order_of(row.at(at)) > order_of(most)) most = row.at(at);
+                }
+                runs[run] = most;
+            }
+            __syncthreads();
+        }
         int chosen;
         if (count > kLpThreads) {
             // sixteen runs together, then the runs of the chosen sixteens
@@ -326,7 +370,7 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(const T* __restric
 }
 
 // The parts of a row, in their order.
-constexpr int kLpJoinWaves = 4;
+constexpr int kLpJoinWaves = 8;
 template <typename T>
 __global__ __launch_bounds__(64 * kLpJoinWaves) void logprobs_join_kernel(const T* __restrict__ logits, int64_t stride, int vocab, int parts, const LpState* __restrict__ states,
                                                                           const uint64_t* __restrict__ keys, LpOut out) {
@@ -339,7 +383,7 @@ __global__ __launch_bounds__(64 * kLpJoinWaves) void logprobs_join_kernel(const 
         const LpState b = states[row_number * parts + i];
         join(a, b);
     }
-    wave_join(a);
+    wave_join(a, lane);
     if (out.top > 0) {
         uint64_t mine = 0;
         for (int i = wave; i < parts; i += kLpJoinWaves) {
@@ -356,10 +400,10 @@ __global__ __launch_bounds__(64 * kLpJoinWaves) void logprobs_join_kernel(const 
 struct LpPlan {
     int per, parts;
 };
-// Workgroups a row: as few as make the runs of one fit its LDS, and until there are four for each compute unit, no part below eight steps of a workgroup's loads.
+// Workgroups a row: as few as make the runs of one fit its LDS, and until there are four for each compute unit, each with a load for every thread.
 LpPlan lp_plan(int dtype, int64_t rows, int64_t vocab, int top) {
     const int64_t per_load = dtype == QMM_F32 ? 4 : 8, loads = (vocab + 2 * per_load - 2) / per_load;  // (of the worst alignment)
-    const int64_t fewest = (loads + 4 * kLpRuns - 1) / (4 * kLpRuns), enough = (4 * (int64_t)compute_units() + rows - 1) / rows, most = std::max<int64_t>(1, loads / (2 * kLpStep));
+    const int64_t fewest = (loads + 4 * kLpRuns - 1) / (4 * kLpRuns), enough = (4 * (int64_t)compute_units() + rows - 1) / rows, most = std::min<int64_t>(64, std::max<int64_t>(1, loads / kLpThreads));
     int64_t parts = std::max(fewest, std::min(enough, most));
     const int64_t per = ((loads + parts - 1) / parts + 3) / 4 * 4;
     parts = (loads + per - 1) / per;

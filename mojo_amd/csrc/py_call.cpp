@@ -492,6 +492,28 @@ const at::Tensor* expert_matrices(const Encoding* e, PyObject* o, int64_t k, int
     return &t;
 }
 
+// The four tensors of a routing on one device.
+struct RoutingTensors {
+    const at::Tensor *ids, *weights, *offsets, *order;
+    bool open(PyObject* ids_o, PyObject* weights_o, PyObject* offsets_o, PyObject* order_o, int device) {
+        ids = gpu_tensor(ids_o, device);
+        if (!ids) return false;
+        device = ids->device().index();
+        weights = gpu_tensor(weights_o, device), offsets = gpu_tensor(offsets_o, device), order = gpu_tensor(order_o, device);
+        return weights && offsets && order && ids->scalar_type() == at::kInt && weights->scalar_type() == at::kFloat && offsets->scalar_type() == at::kInt && order->scalar_type() == at::kInt &&
+               ids->dim() >= 1 && ids->numel() > 0 && weights->sizes() == ids->sizes() && order->dim() == 1 && order->numel() == ids->numel() && offsets->dim() == 1 && offsets->size(0) >= 2;
+    }
+};
+
+// routing_fits(experts, weights, offsets, order): True if they make a routing
+PyObject* py_routing_fits(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    HANDLE_TH_ERRORS
+    RoutingTensors r;
+    if (count != 4 || !r.open(a[0], a[1], a[2], a[3], -1)) return none();
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
 // experts(op, encoding, lhs, rhs, rhs2, routing, residual, out_dtype)
 PyObject* py_experts(PyObject*, PyObject* const* a, Py_ssize_t count) {
     HANDLE_TH_ERRORS
@@ -503,11 +525,9 @@ PyObject* py_experts(PyObject*, PyObject* const* a, Py_ssize_t count) {
     if (!int_of(a[0], 0, 2, op) || !weight_encoding(e) || e->code == QMM_GPTQ || !c.open_lhs(a[2]) || out_type < 0 || !s_routing || (PyObject*)Py_TYPE(a[5]) != s_routing) return none();
     Attr ids_o(a[5], s_experts), weights_o(a[5], s_weights), offsets_o(a[5], s_offsets), order_o(a[5], s_order);
     if (!ids_o.o || !weights_o.o || !offsets_o.o || !order_o.o) return none();
-    const at::Tensor *ids = gpu_tensor(ids_o.o, c.device), *weights = gpu_tensor(weights_o.o, c.device), *offsets = gpu_tensor(offsets_o.o, c.device), *order = gpu_tensor(order_o.o, c.device);
-    if (!ids || !weights || !offsets || !order || ids->scalar_type() != at::kInt || weights->scalar_type() != at::kFloat || offsets->scalar_type() != at::kInt ||
-        order->scalar_type() != at::kInt || ids->dim() < 1 || ids->numel() == 0 || weights->sizes() != ids->sizes() || order->numel() != ids->numel() || offsets->dim() != 1 ||
-        offsets->size(0) < 2 || offsets->size(0) > QMM_MAX_EXPERTS + 1)
-        return none();
+    RoutingTensors rt;
+    if (!rt.open(ids_o.o, weights_o.o, offsets_o.o, order_o.o, c.device) || rt.offsets->size(0) > QMM_MAX_EXPERTS + 1) return none();
+    const at::Tensor *ids = rt.ids, *weights = rt.weights, *offsets = rt.offsets, *order = rt.order;
     const int64_t top = ids->size(-1), tokens = ids->numel() / top, experts = offsets->size(0) - 1;
     const at::Tensor *w = expert_matrices(e, a[3], c.k, experts, c.device), *w2 = expert_matrices(e, a[4], c.k, experts, c.device);
     if (top > QMM_MAX_TOP || !w || !w2 || w->size(1) != w2->size(1)) return none();
@@ -663,6 +683,7 @@ PyMethodDef g_methods[] = {
     method<py_logprobs>("logprobs", "logprobs(logits, tokens, top_k) -> 4 tensors or None"),
     method<py_matmul_logprobs>("matmul_logprobs", "matmul_logprobs(encoding, config, lhs, rhs, tokens, top_k) -> 4 tensors or None"),
     method<py_routing>("routing", "routing(type)"),
+    method<py_routing_fits>("routing_fits", "routing_fits(experts, weights, offsets, order) -> True or None"),
     {nullptr, nullptr, 0, nullptr},
 };
 

@@ -1355,8 +1355,13 @@ int qmm_matmul_experts(int op, int encoding, const qmm_routing* routing, const v
     if (need > 0 && !aligned(workspace, 256)) return fail(QMM_ERR_INVALID, "qmm_matmul_experts: workspace must be 256-byte aligned");
     const bool out_bf16 = flags & QMM_FLAG_OUT_BF16;
     float* const y = sum ? (float*)((char*)workspace + experts_product_bytes(c)) : nullptr;
-    const hipError_t e = qmm::experts_gemm_supported(c, r) ? qmm::launch_experts_gemm(c, r, sum ? (void*)y : out, out_bf16 && !sum, workspace, (hipStream_t)stream)
-                                                          : qmm::launch_experts_rows(c, r, sum ? (void*)y : out, out_bf16 && !sum, workspace, (hipStream_t)stream);
+    if (sum && qmm::experts_sum_small_wanted(c, r))
+        return hip_status(qmm::launch_experts_sum_small(c, r, residual, residual_dtype, out, out_bf16, (hipStream_t)stream), "qmm_matmul_experts(sum of one token)");
+    void* const to = sum ? (void*)y : out;
+    const bool to_bf16 = out_bf16 && !sum;
+    const hipError_t e = qmm::experts_small_wanted(c, r)     ? qmm::launch_experts_small(c, r, to, to_bf16, (hipStream_t)stream)
+                         : qmm::experts_gemm_supported(c, r) ? qmm::launch_experts_gemm(c, r, to, to_bf16, workspace, (hipStream_t)stream)
+                                                             : qmm::launch_experts_rows(c, r, to, to_bf16, workspace, (hipStream_t)stream);
     if (int rc = hip_status(e, "qmm_matmul_experts")) return rc;
     if (!sum) return QMM_OK;
     return hip_status(qmm::launch_experts_combine(r, y, n, residual, residual_dtype, out, out_bf16, (hipStream_t)stream), "qmm_matmul_experts(sum)");

@@ -34,6 +34,9 @@ class ExpertRouting:
     __slots__ = ("experts", "weights", "offsets", "order")
 
     def __init__(self, experts: torch.Tensor, weights: torch.Tensor, offsets: torch.Tensor, order: torch.Tensor):
+        if (_lib._call or _lib.call()).routing_fits(experts, weights, offsets, order):
+            self.experts, self.weights, self.offsets, self.order = experts, weights, offsets, order
+            return
         for t, name, dtype in ((experts, "experts", torch.int32), (weights, "weights", torch.float32), (offsets, "offsets", torch.int32), (order, "order", torch.int32)):
             _require_gpu(t, name)
             if t.dtype != dtype:

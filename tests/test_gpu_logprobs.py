@@ -11,14 +11,16 @@ DEV = "cuda:0"
 
 def check(got, logits, tokens, top):
     """x - m is rounded by u |x - m|; exp, log and the sums of a wavefront's steps, lanes and parts (values of one sign) by some u of the logarithm and of the entropy's terms: 2^6 u of
-    1 + |x - m| + log S (+ the mean of |x - m|, which the entropy is made of)."""
+    1 + |x - m| + log S (+ the mean of |x - m|, which the entropy is made of).  An exponential that is below 2^-126 beside the rounding of m log2 e, up to 2^-24 |m|, may come out as 0: `vocab` of
+    them, times exponents up to 128 in the entropy."""
     want = R.log_probabilities(logits, tokens, top)
     z = logits.double()
     spread = (z.amax(-1) - torch.logsumexp(z, -1)).abs()
     for g, w, size in ((got.logprobs, want[0], want[0].abs()), (got.entropy, want[1], want[1].abs() + spread), *(((got.top_logprobs, want[3], want[3].abs()),) if top else ())):
         g = g.cpu().double()
         assert g.shape == w.shape
-        limit = 2.0 ** 6 * R.U * size + 1e-30
+        least = 128 * z.shape[-1] * 2.0 ** (-126 + z.amax(-1).abs().clamp(max=2.0 ** 30) * 2.0 ** -24)
+        limit = 2.0 ** 6 * R.U * size + least.reshape(-1, *[1] * (size.dim() - 1))
         error = (g - w).abs()
         assert (error <= limit).all(), f"{(error / limit).max():.3g} of the bound"
     if top:
@@ -102,6 +104,27 @@ def test_masked_infinite_and_nan_rows():
     assert lp[2].isnan() and h[2].isnan() and ids[2, 0] == 17
     assert lp[3].isnan() and h[3].isnan() and 4000 not in ids[3]
     assert lp[5].isnan() and h[5].isnan() and ids[5].tolist() == [0, 1, 2, 3, 4]
+
+
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16))
+def test_a_nan_that_signals_hides_nobody(dtype):
+    bits = {torch.float32: (torch.int32, 0x7f800001), torch.bfloat16: (torch.int16, 0x7f81)}[dtype]
+    x = torch.randn(2, 9000, generator=torch.Generator().manual_seed(4)).to(dtype)
+    want = torch.sort(x[1].float(), descending=True, stable=True).indices[:20]
+    raw = x.view(bits[0])
+    for i in want[:8].tolist():  # beside the largest
+        raw[1, i ^ 1] = bits[1]
+    keep = [i for i in torch.sort(torch.where(x[1].isnan(), -torch.inf, x[1].float()), descending=True, stable=True).indices[:20].tolist()]
+    got = logprobs(x.to(DEV), torch.tensor([0, 0], device=DEV), 20)
+    assert got.logprobs[1].isnan() and not got.logprobs[0].isnan() and got.top_ids[1].tolist() == keep
+
+
+@pytest.mark.parametrize("low,high", ((-1.7e38, 1.7e38), (-3.4e38, 5.0), (-2.0, 3.0e38), (-3.4e38, -3.3e38), (1.0e37, 2.0e37), (2.0 ** 30 - 64, 2.0 ** 30), (2.0 ** 24 - 3, 2.0 ** 24 + 2), (-(2.0 ** 27) - 16, -(2.0 ** 27)), (1000.0, 1002.5)))
+def test_values_at_the_ends_of_the_range(low, high):
+    x = torch.full((3, 20000), low)
+    x[0, 7] = x[1, 19999] = x[2, 0] = x[2, 9999] = high
+    tokens = torch.tensor([7, 19999, 9999])
+    check(logprobs(x.to(DEV), tokens.to(DEV), 2), x, tokens, 2)
 
 
 def test_masked_everywhere_but_one_and_alternatives_beyond_the_mask():

@@ -56,7 +56,7 @@ struct RouteCall {
 
 // One token by one wavefront; lane j holds expert 64 i + j in x[i].
 template <int VPL, typename T>
-__device__ __forceinline__ void route_token(const T* __restrict__ logits, const RouteCall& c, int64_t token, int lane, int32_t* __restrict__ ids, float* __restrict__ weights) {
+__device__ __forceinline__ void route_token(const T* __restrict__ logits, const RouteCall& c, int64_t token, int lane, int32_t* __restrict__ ids, float* __restrict__ weights, int* lds_ids) {
     float x[VPL];
 #pragma unroll
     for (int i = 0; i < VPL; i++) {
@@ -145,6 +145,7 @@ __device__ __forceinline__ void route_token(const T* __restrict__ logits, const 
     }
     if (lane < c.top) {
         ids[token * c.top + lane] = expert;
+        if (lds_ids) lds_ids[token * c.top + lane] = expert;
         weights[token * c.top + lane] = w * c.scale;
     }
 }
@@ -237,8 +238,29 @@ template <int VPL, typename T>
 __global__ __launch_bounds__(kRouteThreads) void route_kernel(const T* __restrict__ logits, RouteCall c, int per, int32_t* ids, float* weights, int32_t* offsets, int32_t* order, int32_t* blocks) {
     extern __shared__ int route_lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int t0 = (int)blockIdx.x * per, t1 = min(t0 + per, c.tokens);
-    for (int t = t0 + wave; t < t1; t += kRouteWaves) route_token<VPL>(logits, c, t, lane, ids, weights);
+    const int t0 = (int)blockIdx.x * per, t1 = min(t0 + per, c.tokens), waves = (int)blockDim.x >> 6;
+    __shared__ int few[64];
+    const bool is_few = c.tokens * c.top <= 64;
+    for (int t = t0 + wave; t < t1; t += waves) route_token<VPL>(logits, c, t, lane, ids, weights, is_few ? few : nullptr);
+    if (is_few) {
+        // a pair a lane: its place is the number of pairs before it; every thread counts the pairs of experts below some
+        __syncthreads();
+        const int pairs = c.tokens * c.top, mine = lane < pairs ? few[lane] : 0x7fffffff;
+        if (wave == 0) {
+            int place = 0;
+            for (int i = 0; i < pairs; i++) {
+                const int other = __builtin_amdgcn_readlane(mine, i);
+                place += other < mine || (other == mine && i < lane);
+            }
+            if (lane < pairs) order[place] = lane;
+        }
+        for (int e = threadIdx.x; e <= c.experts; e += (int)blockDim.x) {
+            int below = 0;
+            for (int i = 0; i < pairs; i++) below += __builtin_amdgcn_readlane(mine, i) < e;
+            offsets[e] = below;
+        }
+        return;
+    }
     __threadfence_block();
     __syncthreads();
     count_or_place(ids, t0 * c.top, t1 * c.top, c.experts, route_lds, offsets, order, blocks, wave, lane);
@@ -297,9 +319,10 @@ size_t sort_lds(int experts) { return (size_t)(kRouteWaves + 2) * (experts + 1) 
 
 template <int VPL, typename T>
 hipError_t run_route(const T* logits, const RouteCall& c, int64_t per, int32_t* ids, float* weights, int32_t* offsets, int32_t* order, int32_t* blocks, hipStream_t s) {
-    hipError_t e = allow_full_lds<route_kernel<VPL, T>>();
+    hipError_t e = allow_full_lds<route_kernel<VPL, T>, 256>();
     if (e != hipSuccess) return e;
-    route_kernel<VPL, T><<<dim3((unsigned)((c.tokens + per - 1) / per)), dim3(kRouteThreads), sort_lds(c.experts), s>>>(logits, c, (int)per, ids, weights, offsets, order, blocks);
+    const bool few = (int64_t)c.tokens * c.top <= 64;
+    route_kernel<VPL, T><<<dim3((unsigned)((c.tokens + per - 1) / per)), dim3(few ? 64 * std::min(c.tokens, kRouteWaves) : kRouteThreads), few ? 0 : sort_lds(c.experts), s>>>(logits, c, (int)per, ids, weights, offsets, order, blocks);
     return hipGetLastError();
 }
 template <typename T>

@@ -225,39 +225,19 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(const T* __restric
     const bool wanted = out.top > 0;
 
     const int whole0 = row.skew ? 1 : 0, whole1 = min(end, (row.skew + vocab) / kPer);  // loads that the row fills
-    lp_u4 next[kLpLoads];
-    auto load = [&](int v0) __attribute__((always_inline)) {
-        if (v0 >= whole0 && v0 + 64 * kLpLoads <= whole1) {
-#pragma unroll
-            for (int j = 0; j < kLpLoads; j++) next[j] = *(const lp_u4*)(row.aligned + (int64_t)(v0 + j * 64 + lane) * kPer);
-        } else {
-            constexpr uint32_t kNone = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
-#pragma unroll 1
-            for (int j = 0; j < kLpLoads; j++) {
-                const int v = v0 + j * 64 + lane;
-                lp_u4 raw{kNone, kNone, kNone, kNone};
-                if (v < end) raw = row.whole(v) ? *(const lp_u4*)(row.aligned + (int64_t)v * kPer) : row.edge(v);
-#pragma unroll
-                for (int i = 0; i < kLpLoads; i++) next[i] = i == j ? raw : next[i];
-            }
-        }
-    };
     float m = -__builtin_inff(), f = 0.0f, s = 0.0f, t = 0.0f;  // m and f = m L: of the wavefront; s and t (in units of log 2): of the lane
     int c = 0;                                                  // of the wavefront
-    int v0 = first + wave * 64 * kLpLoads;
-    if (v0 < end) load(v0);
-    for (; v0 < end; v0 += kLpStep) {
+    auto take = [&](int v0, const lp_u4 (&raw)[kLpLoads]) __attribute__((always_inline)) {
         float x[kLpLoads][kPer], most[kLpLoads], all = -__builtin_inff();
 #pragma unroll
         for (int j = 0; j < kLpLoads; j++) {
-            LpRow<T>::unpack(next[j], x[j]);
+            LpRow<T>::unpack(raw[j], x[j]);
             most[j] = x[j][kPer - 1];
 #pragma unroll
             for (int i = 0; i + 1 < kPer - 1; i += 2) most[j] = max3(most[j], x[j][i], x[j][i + 1]);
-            if constexpr (kPer % 2 == 0) most[j] = fmaxf(most[j], x[j][kPer - 2]);
+            most[j] = fmaxf(most[j], x[j][kPer - 2]);
             all = fmaxf(all, most[j]);
         }
-        if (v0 + kLpStep < end) load(v0 + kLpStep);  // on its way meanwhile
         if (wanted) {
             // the maximum of a run, four lanes, is in all of them; lane j of four keeps that of load j
             float keep = 0.0f;
@@ -311,6 +291,42 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(const T* __restric
             }
         s += s2[0] + s2[1];
         t += t2[0] + t2[1];
+    };
+    // this wavefront's steps: those that the row fills, each asked for while the one before is looked at; then the first and the last, which it may not fill
+    const int v_first = first + wave * 64 * kLpLoads;
+    auto fills = [&](int v0) __attribute__((always_inline)) { return v0 >= whole0 && v0 + 64 * kLpLoads <= whole1; };
+    int v0 = v_first < whole0 ? v_first + kLpStep : v_first;
+    if (fills(v0)) {
+        lp_u4 next[kLpLoads];
+        auto load = [&](int v) __attribute__((always_inline)) {
+#pragma unroll
+            for (int j = 0; j < kLpLoads; j++) next[j] = *(const lp_u4*)(row.aligned + (int64_t)(v + j * 64 + lane) * kPer);
+        };
+        load(v0);
+        while (fills(v0)) {
+            lp_u4 raw[kLpLoads];
+#pragma unroll
+            for (int j = 0; j < kLpLoads; j++) raw[j] = next[j];
+            load(fills(v0 + kLpStep) ? v0 + kLpStep : v0);
+            take(v0, raw);
+            v0 += kLpStep;
+        }
+    }
+#pragma unroll 1
+    for (int edge = 0; edge < 2; edge++) {
+        const int v_edge = edge ? v0 : v_first;
+        if (v_edge >= end || (edge == 0 && v_first >= whole0)) continue;
+        constexpr uint32_t kNone = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
+        lp_u4 raw[kLpLoads];
+#pragma unroll 1
+        for (int j = 0; j < kLpLoads; j++) {
+            const int v = v_edge + j * 64 + lane;
+            lp_u4 one{kNone, kNone, kNone, kNone};
+            if (v < end) one = row.whole(v) ? *(const lp_u4*)(row.aligned + (int64_t)v * kPer) : row.edge(v);
+#pragma unroll
+            for (int i = 0; i < kLpLoads; i++) raw[i] = i == j ? one : raw[i];
+        }
+        take(v_edge, raw);
     }
     // f is m L but for its rounding r: every element was 2^r times what it is, with r more in its exponent
     const float r = fabsf(m) <= kLpFar ? fmaf(m, kLog2e, -f) : 0.0f, by = __builtin_amdgcn_exp2f(-r);
@@ -370,11 +386,10 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(const T* __restric
 }
 
 // The parts of a row, in their order.
-constexpr int kLpJoinWaves = 8;
-template <typename T>
-__global__ __launch_bounds__(64 * kLpJoinWaves) void logprobs_join_kernel(const T* __restrict__ logits, int64_t stride, int vocab, int parts, const LpState* __restrict__ states,
+template <typename T, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void logprobs_join_kernel(const T* __restrict__ logits, int64_t stride, int vocab, int parts, const LpState* __restrict__ states,
                                                                           const uint64_t* __restrict__ keys, LpOut out) {
-    __shared__ uint64_t lists[64 * kLpJoinWaves];
+    __shared__ uint64_t lists[64 * WAVES];
     const int lane = threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
     const int64_t row_number = blockIdx.x;
     const LpRow<T> row(logits + row_number * stride, vocab);
@@ -386,13 +401,13 @@ __global__ __launch_bounds__(64 * kLpJoinWaves) void logprobs_join_kernel(const 
     wave_join(a, lane);
     if (out.top > 0) {
         uint64_t mine = 0;
-        for (int i = wave; i < parts; i += kLpJoinWaves) {
+        for (int i = wave; i < parts; i += WAVES) {
             const int at = i == wave ? lane : 63 - lane;
             const uint64_t v = at < out.top ? keys[(row_number * parts + i) * out.top + at] : 0;
             if (i == wave) mine = v;
             else merge64(mine, v, lane);
         }
-        merge_waves<kLpJoinWaves>(mine, lists, wave, lane);
+        merge_waves<WAVES>(mine, lists, wave, lane);
     }
     finish_row(row_number, row, a, lists, out);
 }
@@ -403,7 +418,7 @@ struct LpPlan {
 // Workgroups a row: as few as make the runs of one fit its LDS, and until there are four for each compute unit, each with a load for every thread.
 LpPlan lp_plan(int dtype, int64_t rows, int64_t vocab, int top) {
     const int64_t per_load = dtype == QMM_F32 ? 4 : 8, loads = (vocab + 2 * per_load - 2) / per_load;  // (of the worst alignment)
-    const int64_t fewest = (loads + 4 * kLpRuns - 1) / (4 * kLpRuns), enough = (4 * (int64_t)compute_units() + rows - 1) / rows, most = std::min<int64_t>(64, std::max<int64_t>(1, loads / kLpThreads));
+    const int64_t fewest = (loads + 4 * kLpRuns - 1) / (4 * kLpRuns), enough = (4 * (int64_t)compute_units() + rows / 2) / rows, most = std::min<int64_t>(64, std::max<int64_t>(1, loads / kLpThreads));
     int64_t parts = std::max(fewest, std::min(enough, most));
     const int64_t per = ((loads + parts - 1) / parts + 3) / 4 * 4;
     parts = (loads + per - 1) / per;
@@ -419,7 +434,8 @@ hipError_t run_logprobs(const T* logits, int dtype, int64_t stride, int64_t rows
     logprobs_kernel<T><<<dim3((unsigned)rows, (unsigned)p.parts), dim3(kLpThreads), lds, s>>>(logits, stride, (int)vocab, p.per, p.parts, states, keys, out);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.parts == 1) return e;
-    logprobs_join_kernel<T><<<dim3((unsigned)rows), dim3(64 * kLpJoinWaves), 0, s>>>(logits, stride, (int)vocab, p.parts, states, keys, out);
+    if (p.parts <= 8) logprobs_join_kernel<T, 1><<<dim3((unsigned)rows), dim3(64), 0, s>>>(logits, stride, (int)vocab, p.parts, states, keys, out);
+    else logprobs_join_kernel<T, 8><<<dim3((unsigned)rows), dim3(512), 0, s>>>(logits, stride, (int)vocab, p.parts, states, keys, out);
     return hipGetLastError();
 }
 

@@ -167,7 +167,7 @@ def _matrices(encoding: QuantizationEncoding, t: torch.Tensor, name: str, k: int
 
 
 def _experts(op: int, what: str, encoding, lhs, mats, routing, residual, out_dtype) -> torch.Tensor:
-    done = (_lib._call or _lib.call()).experts(op, encoding, lhs, mats[0], mats[-1], routing, residual, out_dtype)
+    done = (_lib._call or _lib.call()).experts(op, encoding, lhs, mats[0][0], mats[-1][0], routing, residual, out_dtype)
     if done is not None:
         return done
     if not isinstance(encoding, QuantizationEncoding) or not encoding.is_gguf:

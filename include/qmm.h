@@ -326,7 +326,7 @@ int qmm_matmul_experts(int op, int encoding, const qmm_routing* routing, const v
                        int64_t workspace_bytes, int flags, void* stream);
 
 /*
- * Log probabilities of given tokens, entropy and the largest alternatives of rows of logits (fp32 or bf16, row i at logits + i stride values, `vocab` of them):
+ * Log probabilities of given tokens, entropy and the largest alternatives of rows of logits (fp32 or bf16, row i at logits + i stride values, `vocab` of them, up to QMM_MAX_VOCAB):
  *   logprobs[i, c] = x[token] - log sum exp x,  tokens int32 or (tokens_i64) int64[rows, per_row]; a negative token: 0 (padding); one of vocab or more: NaN
  *   entropy[i]     = - sum p log p
  *   top_ids, top_logprobs [rows, top]: the `top` (0 .. 64) largest logits by falling value, equal ones by rising index, NaN below everything
@@ -334,6 +334,7 @@ int qmm_matmul_experts(int op, int encoding, const qmm_routing* routing, const v
  * Workspace: qmm_logprobs_workspace_bytes.
  * qmm_matmul_logprobs is the same of the logits lhs . dequant(rhs)^T (arguments as qmm_matmul; vocab = n), which are kept in the workspace, some rows at a time, and nowhere else.
  */
+#define QMM_MAX_VOCAB (1 << 22)
 int64_t qmm_logprobs_workspace_bytes(int dtype, int64_t rows, int64_t vocab, int top);
 int qmm_logprobs(const void* logits, int dtype, int64_t stride, int64_t rows, int64_t vocab, const void* tokens, int tokens_i64, int per_row, int top, float* logprobs,
                  float* entropy, int32_t* top_ids, float* top_logprobs, void* workspace, int64_t workspace_bytes, void* stream);

@@ -19,6 +19,12 @@ struct ExpertRows {
 
 __device__ __forceinline__ int offset_at(const Routing& r, int e) { return e > r.experts ? r.pairs : min(max(r.offsets[e], 0), r.pairs); }
 
+// The same in scalar registers.  What a load in inline assembly takes as a scalar address must have been worked out there: five wait states lie between a vector instruction that writes a scalar
+// register and a load that reads it, and the compiler, which moves an address over as late as it can, sees no load in the assembly and keeps none of them (such loads fault).
+__device__ __forceinline__ ExpertRows uniform(const ExpertRows& x) {
+    return {__builtin_amdgcn_readfirstlane(x.expert), __builtin_amdgcn_readfirstlane(x.first), __builtin_amdgcn_readfirstlane(x.count)};
+}
+
 // Number `group` of the groups of up to ROWS rows that the experts' runs are cut into, in the order of the experts; count 0: there are not so many.  One wavefront finds it, each lane with a
 // share of the experts.
 template <int ROWS>

@@ -1,9 +1,11 @@
 // The experts' products on the matrix cores: weights packed as they lie in memory, unpacked between the matrix-core instructions, lhs rows gathered by the expert's list.
 //
-// One launch narrows every lhs row to fp16 once (a row's pieces in operand order, next to each other: [K / 64][fp32: hi, residual][8 pieces of 8 columns]); what an expert gets is picked by address, so a
-// token's row is not copied to each of its experts.  Then a workgroup of eight wavefronts takes up to 32 FM rows of one expert's run x 256 columns (gated: 128 of gate and the same 128 of up, whose
-// results meet in LDS): each wavefront unpacks the weights of its 32 columns, the lhs goes global -> LDS directly, a chunk of 64 columns at a time into three buffers that all share.  A load brings
-// eight rows x 128 bytes, lines as memory has them; which of a row's pieces a lane asks for is turned by the row, so that the operands (piece p of 32 rows) are read back without bank conflicts.
+// One launch narrows every lhs row to fp16 once (a row's pieces in operand order, next to each other: [K / 32][fp32: hi, residual][4 pieces of 8 columns]); what an expert gets is picked by address, so a
+// token's row is not copied to each of its experts.  Then a workgroup of four wavefronts takes up to 32 FM rows of one expert's run x 128 columns (gated: 64 of gate and the same 64 of up, whose
+// results meet in LDS): each wavefront unpacks the weights of its 32 columns, the lhs goes global -> LDS directly, a chunk of 32 columns at a time into three or four buffers that all share.  A load brings
+// 16 rows x 64 bytes, as memory has them; which of a row's pieces a lane asks for is turned by the row, so that the operands (piece p of 32 rows) are read back without bank conflicts.
+// LDS is sized for two workgroups on a compute unit: an expert's K is short (8 units of 256 here and there), and what surrounds the products (finding the rows, the way to the first loads, the results) is
+// hidden by the other one.  One workgroup of eight wavefronts x 256 columns instead: 2000 tokens, 8 of 64 experts, 1024 x 2048, Q4_K gate and up 205 us; matrix cores busy a third of the time.
 //
 // The grid counts groups of rows as if every expert's last one were a group more: how many rows an expert has is known on the device only.  A workgroup looks for its group in the offsets
 // (a scan by one wavefront's lanes) and leaves if there is none; a group with few rows runs the body for as many.  Groups of one expert share its weights on one XCD.
@@ -20,7 +22,7 @@ namespace qmm {
 namespace {
 
 struct EgArgs {
-    const uint8_t* a16;    // [lhs rows][k / 64 rounded up to whole units][hi, fp32: residual] of 128 bytes
+    const uint8_t* a16;    // [lhs rows][k / 32 rounded up to whole units][hi, fp32: residual] of 64 bytes
     const uint8_t* sums;   // [lhs rows][units][32 bytes]: sums of 32 columns, eight hi and eight lo parts; Q4_0: eight block scales, zeros
     const float* inv;      // [lhs rows]
     const uint8_t* w[2];
@@ -44,63 +46,76 @@ struct EgQ40 : Q40Weights<1> {
 template <int ENC, bool CENTER>
 using EgWeights = std::conditional_t<ENC == QMM_Q4_0, EgQ40, EgStaged<ENC == QMM_Q4_0 ? QMM_Q4_K : ENC, CENTER>>;
 
-constexpr int kEgWaves = 8, kEgBufs = 3, kEgChunks = 4;  // chunks of 64 columns in a unit of 256
+constexpr int kEgWaves = 4, kEgChunks = 8;  // chunks of 32 columns in a unit of 256
 struct EgRow {
     int64_t at;  // of the row's results, in values; -1: none
     float inv;
     int pad;
 };
+// Rows of a workgroup at most, in 32s: what the registers and half a compute unit's LDS hold.
+constexpr int eg_most(int enc, bool hilo) { return hilo || enc == QMM_Q4_0 ? 2 : 4; }
 template <int ENC, int FM, bool HILO>
 struct EgLds {
     using W = EgWeights<ENC, HILO>;
-    static constexpr int kPer = HILO ? 2 : 1, kChunk = FM * 4096 * kPer, kWeights = kEgWaves * W::kBufs * W::kStage, kSums = W::kMin || W::kQ8 ? 2 * FM * 1024 : 0;
-    static constexpr int kW = kEgBufs * kChunk, kS = kW + kWeights, kResultRow = 40, kResults = kEgWaves * 32 * std::min(FM, 2) * kResultRow * 4;
-    static constexpr int kInfo = std::max(kS + kSums, kResults), kBytes = kInfo + 32 * FM * (int)sizeof(EgRow);
-    static_assert(kBytes <= kLdsPerCu, "fits a compute unit");
+    static constexpr int kPer = HILO ? 2 : 1, kChunk = FM * 2048 * kPer, kWeights = kEgWaves * W::kBufs * W::kStage, kSums = W::kMin || W::kQ8 ? 2 * FM * 1024 : 0;
+    static constexpr int kResultRow = 40, kResults = kEgWaves * 32 * std::min(FM, 2) * kResultRow * 4, kInfoBytes = 32 * FM * (int)sizeof(EgRow);
+    static constexpr int bytes(int bufs) { return std::max(bufs * kChunk + kWeights + kSums, kResults) + kInfoBytes; }
+    static constexpr int kBufs = bytes(4) <= kLdsPerCu / 2 ? 4 : 3;
+    static constexpr int kW = kBufs * kChunk, kS = kW + kWeights, kInfo = std::max(kS + kSums, kResults), kBytes = bytes(kBufs);
+    static_assert(kBytes <= kLdsPerCu / 2, "two on a compute unit");
 };
+
+__device__ __forceinline__ float silu(float v) {
+    // v / (1 + exp(-v)): the product v L as two terms, so that the exponential is right to the last bits for any v
+    const float p = v * -1.44269504088896f, rest = fmaf(v, -1.44269504088896f, -p), e = __builtin_amdgcn_exp2f(p);
+    return v * __builtin_amdgcn_rcpf(1.0f + fmaf(e, rest * 0.693147180559945f, e));
+}
 
 template <int ENC, int FM, bool HILO, bool GATED>
 __device__ __forceinline__ void experts_tile(const EgArgs& p, const Routing& r, const ExpertRows& rows, int col_tile) {
     using W = EgWeights<ENC, HILO>;
     using L = EgLds<ENC, FM, HILO>;
-    constexpr int kPer = L::kPer, kTotal = FM * 4 * kPer, kLoads = (kTotal + kEgWaves - 1) / kEgWaves;  // loads of a chunk, of a wavefront
+    constexpr int kPer = L::kPer, kBufs = L::kBufs, kTotal = FM * 2 * kPer, kLoads = (kTotal + kEgWaves - 1) / kEgWaves;  // loads of a chunk, of a wavefront
     constexpr bool kHasSums = W::kMin || W::kQ8, kUnit = W::kQ8 || (W::kMin && HILO);                   // kUnit: a unit's sums apart from the running ones
     constexpr int kAhead = W::kAhead + (kHasSums ? 1 : 0);
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), row = lane & 31, g = lane >> 5;
-    constexpr int kCols = GATED ? 128 : 256;
-    const int mat = GATED ? wave >> 2 : 0, n0 = col_tile * kCols + 32 * (GATED ? wave & 3 : wave);
+    constexpr int kCols = GATED ? 64 : 128;
+    const int mat = GATED ? wave >> 1 : 0, n0 = col_tile * kCols + 32 * (GATED ? wave & 1 : wave);
     EgRow* const info = (EgRow*)(smem + L::kInfo);
-    auto lhs_row = [&](int i) __attribute__((always_inline)) { return max(pair_at(r, rows.first + min(i, rows.count - 1)), 0) / p.lhs_top; };
-    if (threadIdx.x < 32 * FM) {
-        const int i = (int)threadIdx.x, pair = pair_at(r, rows.first + min(i, rows.count - 1));
-        info[i].at = i < rows.count && pair >= 0 ? (int64_t)pair * p.n : -1;
-        info[i].inv = p.inv[max(pair, 0) / p.lhs_top];
-    }
     WeightTensors wt{p.w[mat] + rows.expert * p.stride[mat], nullptr, nullptr, p.n, p.k, 0};
     const int units = p.units, last_chunk = units * kEgChunks - 1;
     const uint32_t lds0 = lds_address(smem);
-
-    // this wavefront's loads of a chunk: number first + j of them, eight rows each; lane l asks for the piece that belongs at l & 7 of row l >> 3
+    W w;
+    w.init(wt, n0, lane, smem + L::kW + wave * W::kBufs * W::kStage);
+    auto issue_weights = [&](int unit, int buf) __attribute__((always_inline)) {
+        if constexpr (W::kAsync) unrolled<W::kAhead>([&](auto j) __attribute__((always_inline)) { w.template issue<decltype(j)::value>(unit, buf); });
+        else w.load(unit);
+    };
+    auto lhs_row = [&](int i) __attribute__((always_inline)) { return max(pair_at(r, rows.first + min(i, rows.count - 1)), 0) / p.lhs_top; };
+    // this wavefront's loads of a chunk: number first + j of them, 16 rows each; lane l asks for the piece that belongs at l & 3 of row l >> 2
     const int first = min(wave * kLoads, kTotal - kLoads);
     const uint8_t* src[kLoads];
 #pragma unroll
     for (int j = 0; j < kLoads; j++) {
-        const int i = first + j, plane = i / (FM * 4), at_row = i % (FM * 4) * 8 + (lane >> 3), piece = (lane & 7) ^ ((at_row >> 1) & 7);
-        src[j] = p.a16 + (int64_t)lhs_row(at_row) * units * (512 * kPer) + plane * 128 + piece * 16;
+        const int i = first + j, plane = i / (FM * 2), at_row = i % (FM * 2) * 16 + (lane >> 2), piece = (lane & 3) ^ ((at_row >> 2) & 3);
+        src[j] = p.a16 + (int64_t)lhs_row(at_row) * units * (512 * kPer) + plane * 64 + piece * 16;
     }
-    auto issue_lhs = [&](int chunk, int buf) __attribute__((always_inline)) {
-        const int64_t at = (int64_t)min(chunk, last_chunk) * (128 * kPer);
-#pragma unroll
-        for (int j = 0; j < kLoads; j++) load16_to_lds(src[j] + at, (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds0 + buf * L::kChunk + (first + j) * 1024)));
-    };
     const uint8_t* sums_src = nullptr;
     const int sums_tile = wave % FM;
     if constexpr (kHasSums) sums_src = p.sums + (int64_t)lhs_row(32 * sums_tile + row) * units * 32 + g * 16;
-    W w;
-    w.init(wt, n0, lane, smem + L::kW + wave * W::kBufs * W::kStage);
-    auto issue_ahead = [&](int unit, int buf) __attribute__((always_inline)) {
-        if constexpr (W::kAsync) unrolled<W::kAhead>([&](auto j) __attribute__((always_inline)) { w.template issue<decltype(j)::value>(unit, buf); });
+    int info_row = 0;
+    if (threadIdx.x < 32 * FM) {
+        const int pair = pair_at(r, rows.first + min((int)threadIdx.x, rows.count - 1));
+        info_row = max(pair, 0) / p.lhs_top;
+        info[threadIdx.x].at = (int)threadIdx.x < rows.count && pair >= 0 ? (int64_t)pair * p.n : -1;
+    }
+    auto issue_lhs = [&](int chunk, int buf) __attribute__((always_inline)) {
+        const int64_t at = (int64_t)min(chunk, last_chunk) * (64 * kPer);
+#pragma unroll
+        for (int j = 0; j < kLoads; j++) load16_to_lds(src[j] + at, (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds0 + buf * L::kChunk + (first + j) * 1024)));
+    };
+    auto issue_sums = [&](int unit, int buf) __attribute__((always_inline)) {
         if constexpr (kHasSums) load16_to_lds(sums_src + (int64_t)unit * 32, (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds0 + L::kS + (buf * FM + sums_tile) * 1024)));
     };
 
@@ -113,25 +128,26 @@ __device__ __forceinline__ void experts_tile(const EgArgs& p, const Routing& r, 
             if constexpr (kUnit) U[a][i] = 0.0f;
         }
     const float16v zero16 = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    // where a lane's operands of the four steps of a chunk lie
-    uint32_t at_step[4];
+    // where a lane's operands of the two steps of a chunk lie
+    uint32_t at_step[2];
 #pragma unroll
-    for (int t = 0; t < 4; t++) at_step[t] = row * 128 + (((2 * t + g) ^ ((row >> 1) & 7)) << 4);
+    for (int t = 0; t < 2; t++) at_step[t] = row * 64 + (((2 * t + g) ^ ((row >> 2) & 3)) << 4);
     half8 af[2][FM][kPer], b[2][W::kPlanes];
     auto read_lhs = [&](int step, int slot, uint32_t base) __attribute__((always_inline)) {
 #pragma unroll
         for (int a = 0; a < FM; a++)
 #pragma unroll
-            for (int q = 0; q < kPer; q++) af[slot][a][q] = *(const half8*)(smem + base + at_step[step] + (q * FM + a) * 4096);
+            for (int q = 0; q < kPer; q++) af[slot][a][q] = *(const half8*)(smem + base + at_step[step] + (q * FM + a) * 2048);
     };
 
-    if constexpr (!W::kAsync) w.load(0);
-    issue_ahead(0, 0);
-    issue_lhs(0, 0);
-    issue_lhs(1, 1);
-    wait_vmcnt<kLoads>();
+    // (From here on the loads are counted: an ordinary one among them would wait for all.)
+    issue_weights(0, 0);
+    issue_sums(0, 0);
+#pragma unroll
+    for (int c = 0; c < kBufs - 1; c++) issue_lhs(c, c);
+    wait_vmcnt<(kBufs - 2) * kLoads>();
     __syncthreads();
-    issue_lhs(2, 2);
+    issue_lhs(kBufs - 1, kBufs - 1);
     if constexpr (W::kAsync) w.open(0, 0);
     else w.open();
     read_lhs(0, 0, 0);
@@ -141,8 +157,8 @@ __device__ __forceinline__ void experts_tile(const EgArgs& p, const Routing& r, 
     for (int u = 0; u < units; u++) {
         const int next = min(u + 1, units - 1);
         // (nobody reads the sums and weights of the unit before any more)
-        if constexpr (!W::kAsync) w.load(next);
-        issue_ahead(next, (u + 1) & 1);
+        issue_weights(next, (u + 1) & 1);
+        issue_sums(next, (u + 1) & 1);
         float dmin = 0.0f, dnext = 0.0f;
         half8 scales[FM];
         if constexpr (W::kQ8) {
@@ -154,16 +170,17 @@ __device__ __forceinline__ void experts_tile(const EgArgs& p, const Routing& r, 
         }
         __builtin_amdgcn_sched_barrier(0);
         unrolled<16>([&](auto tt) __attribute__((always_inline)) {
-            constexpr int t = decltype(tt)::value, cur = t & 1, chunk = t / 4;
-            if constexpr (t % 4 == 3) {
-                // The next chunk has arrived (asked for two boundaries ago, before the chunk after it; where the next unit's weights were asked for since, they are younger too), and every
-                // wavefront has read this one's operands into registers: its buffer takes the chunk after the two that are there.  At a unit's end the weights are older than the chunk.
-                wait_vmcnt<kLoads + (chunk < 2 ? kAhead : 0)>();
+            constexpr int t = decltype(tt)::value, cur = t & 1, entered = t / 2 + 1;
+            if constexpr (t % 2 == 1) {
+                // The next chunk has arrived (asked for kBufs - 1 boundaries ago; younger: the chunks after it, and the next unit's weights and sums where they were asked for since), and every wavefront has
+                // read this one's operands into registers: its buffer takes the chunk after those that are there.  At a unit's end the weights are older than the chunk.
+                static_assert(kBufs - 1 < kEgChunks, "the weights of the next unit are older than its first chunk");
+                wait_vmcnt<(kBufs - 2) * kLoads + (entered <= kBufs - 1 ? kAhead : 0)>();
                 __syncthreads();
-                issue_lhs(u * kEgChunks + chunk + 3, buf);
-                buf = buf == kEgBufs - 1 ? 0 : buf + 1;
+                issue_lhs(u * kEgChunks + entered + kBufs - 1, buf);
+                buf = buf == kBufs - 1 ? 0 : buf + 1;
             }
-            read_lhs((t + 1) % 4, cur ^ 1, (uint32_t)(buf * L::kChunk));
+            read_lhs((t + 1) % 2, cur ^ 1, (uint32_t)(buf * L::kChunk));
             if constexpr (W::kAsync) {
                 if constexpr (t + 1 == 16) w.open(next, (u + 1) & 1);
             }
@@ -258,9 +275,11 @@ __device__ __forceinline__ void experts_tile(const EgArgs& p, const Routing& r, 
 #pragma unroll
             for (int i = 0; i < 16; i++) T[a][i] = kUnit ? T[a][i] + fmaf(d, P[a][i], U[a][i]) : fmaf(d, P[a][i], T[a][i]);
     }
+    if (threadIdx.x < 32 * FM) info[threadIdx.x].inv = p.inv[info_row];
     wait_vmcnt<0>();
     __syncthreads();  // nothing is on its way into the buffers any more, which now take the results
     constexpr int kRow = L::kResultRow, kTiles = std::min(FM, 2), kTile = 32 * kTiles * kRow;
+    static_assert(FM % kTiles == 0, "every turn has all its rows: beyond the last one `info` holds no place to store to");
     float* const mine = (float*)smem + wave * kTile;
 #pragma unroll
     for (int a0 = 0; a0 < FM; a0 += kTiles) {
@@ -271,10 +290,10 @@ __device__ __forceinline__ void experts_tile(const EgArgs& p, const Routing& r, 
             for (int i = 0; i < 16; i++) mine[(32 * (a - a0) + 8 * (i >> 2) + 4 * g + (i & 3)) * kRow + row] = T[a][i];
         __syncthreads();
         // two rows of 32 columns at a time; gated: the wavefronts of gate take the first half of the rows, those of up the second
-        const int strip = GATED ? wave & 3 : wave, col = col_tile * kCols + 32 * strip + row;
+        const int strip = GATED ? wave & 1 : wave, col = col_tile * kCols + 32 * strip + row;
         const float* const y = (const float*)smem + strip * kTile;
         constexpr int kMine = GATED ? 16 * kTiles : 32 * kTiles;
-        const int from = GATED ? (wave >> 2) * kMine : 0;
+        const int from = GATED ? (wave >> 1) * kMine : 0;
         if (col < p.n) {
             for (int i0 = from + g; i0 < from + kMine; i0 += 8) {
                 EgRow e[4];
@@ -284,7 +303,7 @@ __device__ __forceinline__ void experts_tile(const EgArgs& p, const Routing& r, 
                     const int i = i0 + 2 * j;
                     e[j] = info[32 * a0 + i];
                     v[j] = y[i * kRow + row] * e[j].inv;
-                    if constexpr (GATED) v[j] = v[j] / (1.0f + expf(-v[j])) * (y[4 * kTile + i * kRow + row] * e[j].inv);
+                    if constexpr (GATED) v[j] = silu(v[j]) * (y[2 * kTile + i * kRow + row] * e[j].inv);
                 }
                 if (p.out_bf16) {
 #pragma unroll
@@ -302,7 +321,7 @@ __device__ __forceinline__ void experts_tile(const EgArgs& p, const Routing& r, 
 
 template <bool GATED>
 __device__ __forceinline__ void zero_tile(const EgArgs& p, const Routing& r, const ExpertRows& rows, int col_tile) {
-    constexpr int kCols = GATED ? 128 : 256;
+    constexpr int kCols = GATED ? 64 : 128;
     const int col = col_tile * kCols + (int)threadIdx.x % kCols;
     if (col >= p.n) return;
     for (int i = (int)threadIdx.x / kCols; i < rows.count; i += 64 * kEgWaves / kCols) {
@@ -315,14 +334,14 @@ __device__ __forceinline__ void zero_tile(const EgArgs& p, const Routing& r, con
 
 template <int ENC, int FM, bool HILO, bool GATED>
 __global__ __launch_bounds__(64 * kEgWaves, 2) void experts_gemm_kernel(EgArgs p, Routing r) {
-    const ExpertRows rows = find_rows<32 * FM>(r, (int)blockIdx.y, threadIdx.x & 63);
+    const ExpertRows rows = uniform(find_rows<32 * FM>(r, (int)blockIdx.y, threadIdx.x & 63));
     if (rows.count == 0) return;
     // columns of one expert go over the XCDs, beginning with another one for each
     const int col_tile = (int)blockIdx.z * 8 + (((int)blockIdx.x + rows.expert) & 7);
-    if (col_tile * (GATED ? 128 : 256) >= p.n) return;
+    if (col_tile * (GATED ? 64 : 128) >= p.n) return;
     if (rows.expert >= r.experts) return zero_tile<GATED>(p, r, rows, col_tile);
     if constexpr (FM > 2) {
-        if (rows.count > 64) return experts_tile<ENC, FM, HILO, GATED>(p, r, rows, col_tile);
+        if (rows.count > 64) return experts_tile<ENC, 4, HILO, GATED>(p, r, rows, col_tile);
     }
     if constexpr (FM > 1) {
         if (rows.count > 32) return experts_tile<ENC, 2, HILO, GATED>(p, r, rows, col_tile);
@@ -378,9 +397,9 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void experts_prep_kernel(con
     auto emit = [&](int pc, const LhsPiece<AT>& x) __attribute__((always_inline)) {
         float v[8];
         unpack_piece(x, v);
-        // columns 8 pc ..: block blk of 32, half g, step 2 blk + a: piece 2 (step % 4) + g of chunk step / 4
-        const int blk = pc >> 2, at_g = (pc >> 1) & 1, step = 2 * blk + (pc & 1);
-        uint8_t* const at = to + (step >> 2) * (128 * kPer) + (2 * (step & 3) + at_g) * 16;
+        // columns 8 pc ..: chunk blk, half g, step a: piece 2 a + g
+        const int blk = pc >> 2, at_g = (pc >> 1) & 1;
+        uint8_t* const at = to + blk * (64 * kPer) + (2 * (pc & 1) + at_g) * 16;
         constexpr int perm[8] = {0, 2, 1, 3, 4, 6, 5, 7};
 #pragma unroll
         for (int i = 0; i < 8; i++) v[i] *= s;
@@ -398,7 +417,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void experts_prep_kernel(con
             }
 #pragma unroll
             for (int i = 0; i < 4; i++) lo.u[i] = narrow2(rest[2 * i], rest[2 * i + 1]);
-            *(half8*)(at + 128) = lo.h;
+            *(half8*)(at + 64) = lo.h;
         }
         if (with_sums) {
             float sum = 0.0f;
@@ -430,7 +449,7 @@ __global__ __launch_bounds__(256) void experts_prep_q8_kernel(const AT* __restri
     if (row >= rows) return;  // (whole blocks: a multiple of four threads)
     const int pc = (int)(i - row * (units * 32)), pieces = k >> 3;
     if (pc == 0) inv[row] = 1.0f;
-    const int blk = pc >> 2, sub = pc & 3, g = sub & 1, step = 2 * blk + (sub >> 1);  // columns 32 blk + 16 a + 8 g: step 2 blk + a
+    const int blk = pc >> 2, sub = pc & 3, g = sub & 1;  // columns 32 blk + 16 a + 8 g: step a of chunk blk
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (pc < pieces) unpack_piece(load_piece(a + row * k + pc * 8), v);
     float mx = 0.0f;
@@ -444,7 +463,7 @@ __global__ __launch_bounds__(256) void experts_prep_q8_kernel(const AT* __restri
     gd_u4 o;
 #pragma unroll
     for (int j = 0; j < 4; j++) o[j] = pack_half2((float)q8_0_code(v[perm[2 * j]], id), (float)q8_0_code(v[perm[2 * j + 1]], id));
-    *(gd_u4*)(a16 + row * units * 512 + (step >> 2) * 128 + (2 * (step & 3) + g) * 16) = o;
+    *(gd_u4*)(a16 + row * units * 512 + blk * 64 + (2 * (sub >> 1) + g) * 16) = o;
     if (sub == 0) {
         uint16_t* const sp = (uint16_t*)(sums + (row * units + (blk >> 3)) * 32) + (blk & 7);
         sp[0] = dh;
@@ -484,10 +503,10 @@ hipError_t run_prep(const ExpertCall& c, const EgArgs& p, hipStream_t s) {
 
 template <int ENC, int FM, bool HILO, bool GATED>
 hipError_t run_gemm(const EgArgs& p, const Routing& r, hipStream_t s) {
-    constexpr int lds = std::max(EgLds<ENC, FM, HILO>::kBytes, std::max(EgLds<ENC, 1, HILO>::kBytes, EgLds<ENC, std::min(FM, 2), HILO>::kBytes));
+    constexpr int lds = std::max(std::max(EgLds<ENC, FM, HILO>::kBytes, EgLds<ENC, 1, HILO>::kBytes), EgLds<ENC, std::min(FM, 2), HILO>::kBytes);
     const hipError_t e = allow_full_lds<experts_gemm_kernel<ENC, FM, HILO, GATED>>();
     if (e != hipSuccess) return e;
-    const int cols = GATED ? 128 : 256;
+    const int cols = GATED ? 64 : 128;
     experts_gemm_kernel<ENC, FM, HILO, GATED><<<dim3(8, (unsigned)most_groups(r.pairs, r.experts, 32 * FM), (unsigned)((p.n + 8 * cols - 1) / (8 * cols))), dim3(64 * kEgWaves), lds, s>>>(p, r);
     return hipGetLastError();
 }
@@ -496,20 +515,23 @@ hipError_t run_gemm(const EgArgs& p, const Routing& r, hipStream_t s) {
     return p.gated ? run_gemm<ENC, FM, HILO, true>(p, r, s) : run_gemm<ENC, FM, HILO, false>(p, r, s);
 }
 // rows of a group: 32 fm
+template <int ENC, bool HILO>
+hipError_t run_gemm_rows(const EgArgs& p, const Routing& r, int fm, hipStream_t s) {
+    constexpr int kMost = eg_most(ENC, HILO);
+    return fm == 1 ? run_gemm<ENC, 1, HILO>(p, r, s) : fm == 2 ? run_gemm<ENC, 2, HILO>(p, r, s) : run_gemm<ENC, kMost, HILO>(p, r, s);
+}
 template <int ENC>
 hipError_t run_gemm(const EgArgs& p, const Routing& r, int fm, bool hilo, hipStream_t s) {
     if constexpr (ENC != QMM_Q4_0) {
-        if (hilo) return fm == 1 ? run_gemm<ENC, 1, true>(p, r, s) : run_gemm<ENC, 2, true>(p, r, s);
-        if (fm == 4) return run_gemm<ENC, 4, false>(p, r, s);
+        if (hilo) return run_gemm_rows<ENC, true>(p, r, fm, s);
     }
-    return fm == 1 ? run_gemm<ENC, 1, false>(p, r, s) : run_gemm<ENC, 2, false>(p, r, s);
+    return run_gemm_rows<ENC, false>(p, r, fm, s);
 }
 
 // Rows of a group, in 32s: as many as an expert has on average, up to what the registers hold.
 int eg_rows(const ExpertCall& c, const Routing& r) {
     const int64_t mean = r.pairs / r.experts;
-    const int most = c.encoding == QMM_Q4_0 || c.lhs_dtype == QMM_F32 ? 2 : 4;
-    return std::min(mean <= 32 ? 1 : mean <= 64 ? 2 : 4, most);
+    return std::min(mean <= 32 ? 1 : mean <= 64 ? 2 : 4, eg_most(c.encoding, c.lhs_dtype == QMM_F32));
 }
 
 }  // namespace

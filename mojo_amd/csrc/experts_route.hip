@@ -54,9 +54,9 @@ struct RouteCall {
     const float* bias;
 };
 
-// One token by one wavefront; lane j holds expert 64 i + j in x[i].
+// One token by one wavefront; lane j holds expert 64 i + j in x[i].  Its j-th expert, in lane j.
 template <int VPL, typename T>
-__device__ __forceinline__ void route_token(const T* __restrict__ logits, const RouteCall& c, int64_t token, int lane, int32_t* __restrict__ ids, float* __restrict__ weights, int* lds_ids) {
+__device__ __forceinline__ int route_token(const T* __restrict__ logits, const RouteCall& c, int64_t token, int lane, int32_t* __restrict__ ids, float* __restrict__ weights) {
     float x[VPL];
 #pragma unroll
     for (int i = 0; i < VPL; i++) {
@@ -145,9 +145,9 @@ __device__ __forceinline__ void route_token(const T* __restrict__ logits, const 
     }
     if (lane < c.top) {
         ids[token * c.top + lane] = expert;
-        if (lds_ids) lds_ids[token * c.top + lane] = expert;
         weights[token * c.top + lane] = w * c.scale;
     }
+    return expert;
 }
 
 // LDS of the sort: counts[wavefronts][experts + 1], then start[experts + 1]
@@ -238,32 +238,45 @@ template <int VPL, typename T>
 __global__ __launch_bounds__(kRouteThreads) void route_kernel(const T* __restrict__ logits, RouteCall c, int per, int32_t* ids, float* weights, int32_t* offsets, int32_t* order, int32_t* blocks) {
     extern __shared__ int route_lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int t0 = (int)blockIdx.x * per, t1 = min(t0 + per, c.tokens), waves = (int)blockDim.x >> 6;
-    __shared__ int few[64];
-    const bool is_few = c.tokens * c.top <= 64;
-    for (int t = t0 + wave; t < t1; t += waves) route_token<VPL>(logits, c, t, lane, ids, weights, is_few ? few : nullptr);
-    if (is_few) {
-        // a pair a lane: its place is the number of pairs before it; every thread counts the pairs of experts below some
-        __syncthreads();
-        const int pairs = c.tokens * c.top, mine = lane < pairs ? few[lane] : 0x7fffffff;
-        if (wave == 0) {
-            int place = 0;
-            for (int i = 0; i < pairs; i++) {
-                const int other = __builtin_amdgcn_readlane(mine, i);
-                place += other < mine || (other == mine && i < lane);
-            }
-            if (lane < pairs) order[place] = lane;
-        }
-        for (int e = threadIdx.x; e <= c.experts; e += (int)blockDim.x) {
-            int below = 0;
-            for (int i = 0; i < pairs; i++) below += __builtin_amdgcn_readlane(mine, i) < e;
-            offsets[e] = below;
-        }
-        return;
-    }
+    const int t0 = (int)blockIdx.x * per, t1 = min(t0 + per, c.tokens);
+    for (int t = t0 + wave; t < t1; t += kRouteWaves) route_token<VPL>(logits, c, t, lane, ids, weights);
     __threadfence_block();
     __syncthreads();
     count_or_place(ids, t0 * c.top, t1 * c.top, c.experts, route_lds, offsets, order, blocks, wave, lane);
+}
+
+// Up to 64 pairs in all: one a lane.  Its place is the number of pairs before it; every thread counts the pairs of experts below some.
+template <int VPL, typename T>
+__global__ __launch_bounds__(kRouteThreads) void route_few_kernel(const T* __restrict__ logits, RouteCall c, int32_t* __restrict__ ids, float* __restrict__ weights, int32_t* __restrict__ offsets,
+                                                                  int32_t* __restrict__ order) {
+    __shared__ int few[64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), pairs = c.tokens * c.top;
+    int mine;
+    if (c.tokens == 1) {
+        mine = route_token<VPL>(logits, c, 0, lane, ids, weights);
+    } else {
+        for (int t = wave; t < c.tokens; t += (int)blockDim.x >> 6) {
+            const int expert = route_token<VPL>(logits, c, t, lane, ids, weights);
+            if (lane < c.top) few[t * c.top + lane] = expert;
+        }
+        __syncthreads();
+        mine = few[lane];
+    }
+    if (lane >= pairs) mine = 0x7fffffff;
+    if (wave == 0) {
+        int place = 0;
+        for (int i = 0; i < pairs; i++) {
+            const int other = __builtin_amdgcn_readlane(mine, i);
+            place += other < mine || (other == mine && i < lane);
+        }
+        if (lane < pairs) order[place] = lane;
+    }
+    for (int e0 = 0; e0 <= c.experts; e0 += (int)blockDim.x) {
+        const int e = e0 + (int)threadIdx.x;
+        int below = 0;
+        for (int i = 0; i < pairs; i++) below += __builtin_amdgcn_readlane(mine, i) < e;
+        if (e <= c.experts) offsets[e] = below;
+    }
 }
 
 __global__ __launch_bounds__(kRouteThreads) void group_kernel(const int32_t* __restrict__ ids, int pairs, int experts, int per, int32_t* offsets, int32_t* order, int32_t* blocks) {
@@ -282,16 +295,16 @@ __global__ __launch_bounds__(kRouteThreads) void place_kernel(const int32_t* __r
     int* const before = start + runs;
     for (int e = threadIdx.x; e < runs; e += kRouteThreads) start[e] = before[e] = 0;
     __syncthreads();
-    // the counts of all workgroups and of those before this one: as many threads share an expert's as there are, each eight loads at a time
+    // the counts of all workgroups and of those before this one: as many threads share an expert's as there are, each 32 loads at a time
     const int width = (runs + 63) / 64 * 64, shares = max(1, kRouteThreads / width), blocks_all = (int)gridDim.x;
     for (int e = (int)threadIdx.x % width; e < runs && (int)threadIdx.x < shares * width; e += kRouteThreads) {
         int sum = 0, mine = 0;
-        for (int b0 = (int)threadIdx.x / width; b0 < blocks_all; b0 += 8 * shares) {
-            int v[8];
+        for (int b0 = (int)threadIdx.x / width; b0 < blocks_all; b0 += 32 * shares) {
+            int v[32];
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = b0 + i * shares < blocks_all ? blocks[(int64_t)(b0 + i * shares) * runs + e] : 0;
+            for (int i = 0; i < 32; i++) v[i] = b0 + i * shares < blocks_all ? blocks[(int64_t)(b0 + i * shares) * runs + e] : 0;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
+            for (int i = 0; i < 32; i++) {
                 sum += v[i];
                 mine += b0 + i * shares < (int)blockIdx.x ? v[i] : 0;
             }
@@ -319,10 +332,13 @@ size_t sort_lds(int experts) { return (size_t)(kRouteWaves + 2) * (experts + 1) 
 
 template <int VPL, typename T>
 hipError_t run_route(const T* logits, const RouteCall& c, int64_t per, int32_t* ids, float* weights, int32_t* offsets, int32_t* order, int32_t* blocks, hipStream_t s) {
-    hipError_t e = allow_full_lds<route_kernel<VPL, T>, 256>();
+    if ((int64_t)c.tokens * c.top <= 64) {
+        route_few_kernel<VPL, T><<<dim3(1), dim3((unsigned)(64 * std::min(c.tokens, kRouteWaves))), 0, s>>>(logits, c, ids, weights, offsets, order);
+        return hipGetLastError();
+    }
+    hipError_t e = allow_full_lds<route_kernel<VPL, T>>();
     if (e != hipSuccess) return e;
-    const bool few = (int64_t)c.tokens * c.top <= 64;
-    route_kernel<VPL, T><<<dim3((unsigned)((c.tokens + per - 1) / per)), dim3(few ? 64 * std::min(c.tokens, kRouteWaves) : kRouteThreads), few ? 0 : sort_lds(c.experts), s>>>(logits, c, (int)per, ids, weights, offsets, order, blocks);
+    route_kernel<VPL, T><<<dim3((unsigned)((c.tokens + per - 1) / per)), dim3(kRouteThreads), sort_lds(c.experts), s>>>(logits, c, (int)per, ids, weights, offsets, order, blocks);
     return hipGetLastError();
 }
 template <typename T>

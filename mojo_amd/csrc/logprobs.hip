@@ -42,6 +42,10 @@ __device__ __forceinline__ uint32_t order_of(float x) {
 }
 __device__ __forceinline__ uint64_t key_of(float x, uint32_t index) { return (uint64_t)order_of(x) << 32 | (uint32_t)~index; }
 __device__ __forceinline__ uint32_t index_of(uint64_t key) { return ~(uint32_t)key; }
+__device__ __forceinline__ float value_of(uint64_t key) {  // (a NaN comes out as one)
+    const uint32_t o = (uint32_t)(key >> 32);
+    return __uint_as_float((o & 0x80000000u) ? o ^ 0x80000000u : ~o);
+}
 
 constexpr float kLog2e = 1.44269504088896f, kLn2 = 0.693147180559945f;
 __device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }  // d <= 0
@@ -191,22 +195,32 @@ struct LpOut {
     int top;
 };
 
-// What a row's state says.  lists: its `top` largest keys.
+// A token of a row and its logit, asked for before the row is looked at.
+struct LpToken {
+    int64_t token;
+    float x;
+};
 template <typename T>
-__device__ __forceinline__ void finish_row(int64_t row_number, const LpRow<T>& row, const LpState& a, const uint64_t* lists, const LpOut& out) {
+__device__ __forceinline__ LpToken token_at(int64_t row_number, const LpRow<T>& row, int i, const LpOut& out) {
+    const int64_t at = row_number * out.per_row + i, token = out.wide ? ((const int64_t*)out.tokens)[at] : ((const int32_t*)out.tokens)[at];
+    return {token, token >= 0 && token < row.vocab ? row.at(token) : 0.0f};
+}
+// What a row's state says.  mine: the thread's token (the first `blockDim` of the row's have one each); lists: the row's `top` largest keys.
+template <typename T>
+__device__ __forceinline__ void finish_row(int64_t row_number, const LpRow<T>& row, const LpState& a, LpToken mine, const uint64_t* lists, const LpOut& out) {
     const float rest = (float)(a.c - 1) + a.s, log_total = log1pf(rest);
     const bool none = a.m == -__builtin_inff() && !(a.s != a.s);  // no mass at all
     const float bad = a.m == __builtin_inff() ? __builtin_nanf("") : 0.0f;
     auto log_p = [&](float x) { return none ? -__builtin_inff() : (x - a.m) - log_total + bad; };
     for (int i = threadIdx.x; i < out.per_row; i += (int)blockDim.x) {
-        const int64_t at = row_number * out.per_row + i, token = out.wide ? ((const int64_t*)out.tokens)[at] : ((const int32_t*)out.tokens)[at];
-        out.chosen[at] = token < 0 ? 0.0f : token >= row.vocab ? __builtin_nanf("") : log_p(row.at(token));
+        if (i >= (int)blockDim.x) mine = token_at(row_number, row, i, out);
+        out.chosen[row_number * out.per_row + i] = mine.token < 0 ? 0.0f : mine.token >= row.vocab ? __builtin_nanf("") : log_p(mine.x);
     }
     if (threadIdx.x == 0) out.entropy[row_number] = none ? 0.0f : log_total - a.t / ((float)a.c + a.s) + bad;
     if ((int)threadIdx.x < out.top) {
-        const uint32_t id = index_of(lists[threadIdx.x]);
-        out.top_ids[row_number * out.top + threadIdx.x] = (int32_t)id;
-        out.top_values[row_number * out.top + threadIdx.x] = log_p(row.at(id));
+        const uint64_t key = lists[threadIdx.x];
+        out.top_ids[row_number * out.top + threadIdx.x] = (int32_t)index_of(key);
+        out.top_values[row_number * out.top + threadIdx.x] = log_p(value_of(key));
     }
 }
 
@@ -223,6 +237,8 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(const T* __restric
     const LpRow<T> row(logits + row_number * stride, vocab);
     const int first = part * per, end = min(first + per, row.loads());
     const bool wanted = out.top > 0;
+    LpToken token{0, 0.0f};
+    if (parts == 1 && (int)threadIdx.x < out.per_row) token = token_at(row_number, row, threadIdx.x, out);
 
     const int whole0 = row.skew ? 1 : 0, whole1 = min(end, (row.skew + vocab) / kPer);  // loads that the row fills
     float m = -__builtin_inff(), f = 0.0f, s = 0.0f, t = 0.0f;  // m and f = m L: of the wavefront; s and t (in units of log 2): of the lane
@@ -379,7 +395,7 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(const T* __restric
             return at >= 0 && at < vocab && at < (int64_t)end * kPer - row.skew ? key_of(row.at(at), (uint32_t)at) : 0;
         });
     }
-    if (parts == 1) return finish_row(row_number, row, a, lists, out);
+    if (parts == 1) return finish_row(row_number, row, a, token, lists, out);
     const int64_t place = row_number * parts + part;
     if (threadIdx.x == 0) states[place] = a;
     if ((int)threadIdx.x < out.top) keys[place * out.top + threadIdx.x] = lists[threadIdx.x];
@@ -393,6 +409,8 @@ __global__ __launch_bounds__(64 * WAVES) void logprobs_join_kernel(const T* __re
     const int lane = threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
     const int64_t row_number = blockIdx.x;
     const LpRow<T> row(logits + row_number * stride, vocab);
+    LpToken token{0, 0.0f};
+    if ((int)threadIdx.x < out.per_row) token = token_at(row_number, row, threadIdx.x, out);
     LpState a{-__builtin_inff(), 0.0f, 0.0f, 0};
     for (int i = lane; i < parts; i += 64) {
         const LpState b = states[row_number * parts + i];
@@ -400,22 +418,26 @@ __global__ __launch_bounds__(64 * WAVES) void logprobs_join_kernel(const T* __re
     }
     wave_join(a, lane);
     if (out.top > 0) {
-        uint64_t mine = 0;
-        for (int i = wave; i < parts; i += WAVES) {
-            const int at = i == wave ? lane : 63 - lane;
-            const uint64_t v = at < out.top ? keys[(row_number * parts + i) * out.top + at] : 0;
-            if (i == wave) mine = v;
-            else merge64(mine, v, lane);
+        constexpr int kLists = 64 / WAVES > 8 ? 8 : 64 / WAVES;  // parts <= kLists WAVES
+        uint64_t v[kLists];
+#pragma unroll
+        for (int i = 0; i < kLists; i++) {
+            const int part = wave + i * WAVES, at = i == 0 ? lane : 63 - lane;
+            v[i] = part < parts && at < out.top ? keys[(row_number * parts + part) * out.top + at] : 0;
         }
+        uint64_t mine = v[0];
+#pragma unroll
+        for (int i = 1; i < kLists; i++)
+            if (wave + i * WAVES < parts) merge64(mine, v[i], lane);
         merge_waves<WAVES>(mine, lists, wave, lane);
     }
-    finish_row(row_number, row, a, lists, out);
+    finish_row(row_number, row, a, token, lists, out);
 }
 
 struct LpPlan {
     int per, parts;
 };
-// Workgroups a row: as few as make the runs of one fit its LDS, and until there are four for each compute unit, each with a load for every thread.
+// Workgroups a row: as few as make the runs of one fit its LDS (33 for QMM_MAX_VOCAB fp32 values), and until there are four for each compute unit, each with a load for every thread; 64 at most.
 LpPlan lp_plan(int dtype, int64_t rows, int64_t vocab, int top) {
     const int64_t per_load = dtype == QMM_F32 ? 4 : 8, loads = (vocab + 2 * per_load - 2) / per_load;  // (of the worst alignment)
     const int64_t fewest = (loads + 4 * kLpRuns - 1) / (4 * kLpRuns), enough = (4 * (int64_t)compute_units() + rows / 2) / rows, most = std::min<int64_t>(64, std::max<int64_t>(1, loads / kLpThreads));

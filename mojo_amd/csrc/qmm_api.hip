@@ -1376,7 +1376,7 @@ int64_t qmm_logprobs_workspace_bytes(int dtype, int64_t rows, int64_t vocab, int
 static int check_logprobs(const char* name, int64_t rows, int64_t vocab, const void* tokens, int per_row, int top, const void* logprobs, const void* entropy, const void* top_ids,
                           const void* top_logprobs) {
     if (!entropy || (per_row > 0 && (!tokens || !logprobs)) || (top > 0 && (!top_ids || !top_logprobs))) return fail(QMM_ERR_INVALID, "%s: null pointer", name);
-    if (rows < 1 || rows > INT32_MAX || vocab < 1 || vocab > (1 << 30)) return fail(QMM_ERR_INVALID, "%s: %lld rows of %lld logits", name, (long long)rows, (long long)vocab);
+    if (rows < 1 || rows > INT32_MAX || vocab < 1 || vocab > QMM_MAX_VOCAB) return fail(QMM_ERR_INVALID, "%s: %lld rows of %lld logits", name, (long long)rows, (long long)vocab);
     if (per_row < 0 || top < 0 || top > QMM_MAX_TOP || top > vocab)
         return fail(QMM_ERR_INVALID, "%s: %d tokens a row, %d alternatives of %lld (at most %d)", name, per_row, top, (long long)vocab, QMM_MAX_TOP);
     return QMM_OK;

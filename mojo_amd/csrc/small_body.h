@@ -76,7 +76,7 @@ __device__ __forceinline__ void small_body(const MmMats& mats, const AT* __restr
         part = (int)blockIdx.z;  // (0; the compiler, told so, takes the loop over the groups of K apart and spills)
         er = ex.r.pairs == ex.r.top ? ExpertRows{ex.r.ids[blockIdx.y], (int)blockIdx.y, 1} : find_rows<MROWS>(ex.r, (int)blockIdx.y, lane);  // (one token: a group for each pair, in their order)
         const bool one = ex.r.pairs == ex.r.top;
-        er = {__builtin_amdgcn_readfirstlane(er.expert), __builtin_amdgcn_readfirstlane(er.first), __builtin_amdgcn_readfirstlane(er.count)};
+        er = uniform(er);
         if (er.count == 0) return;
         m = er.count;
         const int listed = one ? er.first : pair_at(ex.r, er.first + min(lane & 15, er.count - 1));

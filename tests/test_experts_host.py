@@ -58,7 +58,7 @@ def test_logprobs_refusals(lib):
     def call(logits=P, dtype=0, stride=100, rows=4, vocab=100, tokens=P, per_row=1, top=3, lp=P, h=P, ids=P, values=P, ws=None, ws_bytes=0):
         return lib.qmm_logprobs(logits, dtype, stride, rows, vocab, tokens, 1, per_row, top, lp, h, ids, values, ws, ws_bytes, None)
 
-    for kw in ({"logits": None}, {"dtype": 2}, {"stride": 99}, {"rows": 0}, {"vocab": 0}, {"vocab": (1 << 30) + 1, "stride": 1 << 31}, {"tokens": None}, {"per_row": -1}, {"top": 65}, {"top": -1},
+    for kw in ({"logits": None}, {"dtype": 2}, {"stride": 99}, {"rows": 0}, {"vocab": 0}, {"vocab": (1 << 22) + 1, "stride": 1 << 31}, {"tokens": None}, {"per_row": -1}, {"top": 65}, {"top": -1},
                {"vocab": 2}, {"lp": None}, {"h": None}, {"ids": None}, {"values": None}, {"logits": C.c_void_p(4098)}):
         assert call(**kw) == -1 and "qmm_logprobs" in message(lib), kw
     need = lib.qmm_logprobs_workspace_bytes(0, 1, 128256, 20)

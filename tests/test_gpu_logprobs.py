@@ -27,7 +27,7 @@ def check(got, logits, tokens, top):
         assert torch.equal(got.top_ids.cpu(), want[2])
 
 
-SHAPES = ((1, 1), (1, 7), (3, 64), (2, 1000), (5, 4097), (700, 33), (1, 32000), (3, 50257), (2, 128256), (130, 8200), (1, 300001))
+SHAPES = ((1, 1), (1, 7), (3, 64), (2, 1000), (5, 4097), (700, 33), (1, 32000), (3, 50257), (2, 128256), (130, 8200), (1, 300001), (1, 2 ** 22))
 
 
 @pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16))

@@ -26,9 +26,9 @@ __device__ __forceinline__ ExpertRows uniform(const ExpertRows& x) {
 }
 
 // Number `group` of the groups of up to ROWS rows that the experts' runs are cut into, in the order of the experts; count 0: there are not so many.  One wavefront finds it, each lane with a
-// share of the experts.
-template <int ROWS>
-__device__ __forceinline__ ExpertRows find_rows(const Routing& r, int group, int lane) {
+// share of the experts.  number(all): the wanted group's number, given how many there are.
+template <int ROWS, typename F>
+__device__ __forceinline__ ExpertRows find_rows_of(const Routing& r, int lane, F&& number) {
     const int per = r.experts / 64 + 1;  // (one run more than there are experts)
     int mine = 0;
     for (int i = 0, at = lane * per; i < per && at <= r.experts; i++, at++) mine += (max(offset_at(r, at + 1) - offset_at(r, at), 0) + ROWS - 1) / ROWS;
@@ -38,7 +38,8 @@ __device__ __forceinline__ ExpertRows find_rows(const Routing& r, int group, int
         const int o = __shfl_up(sum, d);
         if (lane >= d) sum += o;
     }
-    const uint64_t beyond = __ballot(sum > group);
+    const int group = number(__shfl(sum, 63));
+    const uint64_t beyond = group < 0 ? 0 : __ballot(sum > group);
     if (beyond == 0) return {0, 0, 0};
     const int owner = __builtin_ctzll(beyond);
     int left = group - (__shfl(sum, owner) - __shfl(mine, owner)), e = owner * per;
@@ -48,6 +49,10 @@ __device__ __forceinline__ ExpertRows find_rows(const Routing& r, int group, int
         left -= groups;
     }
     return {0, 0, 0};
+}
+template <int ROWS>
+__device__ __forceinline__ ExpertRows find_rows(const Routing& r, int group, int lane) {
+    return find_rows_of<ROWS>(r, lane, [&](int) { return group; });
 }
 // At most so many groups: every run but ends with one that may not be full.
 inline int64_t most_groups(int64_t pairs, int experts, int rows) { return pairs / rows + experts + 1 < pairs ? pairs / rows + experts + 1 : pairs; }

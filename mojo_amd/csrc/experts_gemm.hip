@@ -8,7 +8,7 @@
 // hidden by the other one.  One workgroup of eight wavefronts x 256 columns instead: 2000 tokens, 8 of 64 experts, 1024 x 2048, Q4_K gate and up 205 us; matrix cores busy a third of the time.
 //
 // The grid counts groups of rows as if every expert's last one were a group more: how many rows an expert has is known on the device only.  A workgroup looks for its group in the offsets
-// (a scan by one wavefront's lanes) and leaves if there is none; a group with few rows runs the body for as many.  Groups of one expert share its weights on one XCD.
+// (a scan by one wavefront's lanes) and leaves if there is none; a group with few rows runs the body for as many.
 //
 // Arithmetic as in gemm_staged.hip: exact products of integer codes and fp16 values, fp32 sums, scales applied to the sums of a scale block.
 #include <algorithm>
@@ -46,7 +46,9 @@ struct EgQ40 : Q40Weights<1> {
 template <int ENC, bool CENTER>
 using EgWeights = std::conditional_t<ENC == QMM_Q4_0, EgQ40, EgStaged<ENC == QMM_Q4_0 ? QMM_Q4_K : ENC, CENTER>>;
 
-constexpr int kEgWaves = 4, kEgChunks = 8;  // chunks of 32 columns in a unit of 256
+constexpr int kEgWaves = 4;
+// Steps of 16 columns in a chunk: a barrier for each chunk.
+constexpr int eg_steps(int enc) { return enc == QMM_Q4_K || enc == QMM_Q4_0 ? 4 : 2; }
 struct EgRow {
     int64_t at;  // of the row's results, in values; -1: none
     float inv;
@@ -57,10 +59,10 @@ constexpr int eg_most(int enc, bool hilo) { return hilo || enc == QMM_Q4_0 ? 2 :
 template <int ENC, int FM, bool HILO>
 struct EgLds {
     using W = EgWeights<ENC, HILO>;
-    static constexpr int kPer = HILO ? 2 : 1, kChunk = FM * 2048 * kPer, kWeights = kEgWaves * W::kBufs * W::kStage, kSums = W::kMin || W::kQ8 ? 2 * FM * 1024 : 0;
+    static constexpr int kPer = HILO ? 2 : 1, kSteps = eg_steps(ENC), kChunk = FM * 1024 * kSteps * kPer, kWeights = kEgWaves * W::kBufs * W::kStage, kSums = W::kMin || W::kQ8 ? 2 * FM * 1024 : 0;
     static constexpr int kResultRow = 40, kResults = kEgWaves * 32 * std::min(FM, 2) * kResultRow * 4, kInfoBytes = 32 * FM * (int)sizeof(EgRow);
     static constexpr int bytes(int bufs) { return std::max(bufs * kChunk + kWeights + kSums, kResults) + kInfoBytes; }
-    static constexpr int kBufs = bytes(4) <= kLdsPerCu / 2 ? 4 : 3;
+    static constexpr int kBufs = bytes(4) <= kLdsPerCu / 2 ? 4 : bytes(3) <= kLdsPerCu / 2 ? 3 : 2;
     static constexpr int kW = kBufs * kChunk, kS = kW + kWeights, kInfo = std::max(kS + kSums, kResults), kBytes = bytes(kBufs);
     static_assert(kBytes <= kLdsPerCu / 2, "two on a compute unit");
 };
@@ -75,7 +77,7 @@ template <int ENC, int FM, bool HILO, bool GATED>
 __device__ __forceinline__ void experts_tile(const EgArgs& p, const Routing& r, const ExpertRows& rows, int col_tile) {
     using W = EgWeights<ENC, HILO>;
     using L = EgLds<ENC, FM, HILO>;
-    constexpr int kPer = L::kPer, kBufs = L::kBufs, kTotal = FM * 2 * kPer, kLoads = (kTotal + kEgWaves - 1) / kEgWaves;  // loads of a chunk, of a wavefront
+    constexpr int kPer = L::kPer, kBufs = L::kBufs, kSteps = L::kSteps, kChunks = 16 / kSteps, kTotal = FM * kSteps * kPer, kLoads = (kTotal + kEgWaves - 1) / kEgWaves;  // loads of a chunk, of a wavefront
     constexpr bool kHasSums = W::kMin || W::kQ8, kUnit = W::kQ8 || (W::kMin && HILO);                   // kUnit: a unit's sums apart from the running ones
     constexpr int kAhead = W::kAhead + (kHasSums ? 1 : 0);
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
@@ -84,7 +86,7 @@ __device__ __forceinline__ void experts_tile(const EgArgs& p, const Routing& r, 
     const int mat = GATED ? wave >> 1 : 0, n0 = col_tile * kCols + 32 * (GATED ? wave & 1 : wave);
     EgRow* const info = (EgRow*)(smem + L::kInfo);
     WeightTensors wt{p.w[mat] + rows.expert * p.stride[mat], nullptr, nullptr, p.n, p.k, 0};
-    const int units = p.units, last_chunk = units * kEgChunks - 1;
+    const int units = p.units, last_chunk = units * kChunks - 1;
     const uint32_t lds0 = lds_address(smem);
     W w;
     w.init(wt, n0, lane, smem + L::kW + wave * W::kBufs * W::kStage);
@@ -93,13 +95,16 @@ __device__ __forceinline__ void experts_tile(const EgArgs& p, const Routing& r, 
         else w.load(unit);
     };
     auto lhs_row = [&](int i) __attribute__((always_inline)) { return max(pair_at(r, rows.first + min(i, rows.count - 1)), 0) / p.lhs_top; };
-    // this wavefront's loads of a chunk: number first + j of them, 16 rows each; lane l asks for the piece that belongs at l & 3 of row l >> 2
+    // a row of a chunk is kPieces of 16 bytes; a piece's place is turned by the row, so that the same piece of 16 rows lies in all banks
+    constexpr int kPieces = 2 * kSteps, kRows = 64 / kPieces;  // rows of a load
+    auto turned = [&](int piece, int of_row) __attribute__((always_inline)) { return piece ^ ((of_row * kPieces >> 4) & (kPieces - 1)); };
+    // this wavefront's loads of a chunk: number first + j of them, kRows rows each
     const int first = min(wave * kLoads, kTotal - kLoads);
     const uint8_t* src[kLoads];
 #pragma unroll
     for (int j = 0; j < kLoads; j++) {
-        const int i = first + j, plane = i / (FM * 2), at_row = i % (FM * 2) * 16 + (lane >> 2), piece = (lane & 3) ^ ((at_row >> 2) & 3);
-        src[j] = p.a16 + (int64_t)lhs_row(at_row) * units * (512 * kPer) + plane * 64 + piece * 16;
+        const int i = first + j, plane = i / (FM * kSteps), at_row = i % (FM * kSteps) * kRows + lane / kPieces;
+        src[j] = p.a16 + (int64_t)lhs_row(at_row) * units * (512 * kPer) + plane * (32 * kSteps) + turned(lane % kPieces, at_row) * 16;
     }
     const uint8_t* sums_src = nullptr;
     const int sums_tile = wave % FM;
@@ -111,7 +116,7 @@ __device__ __forceinline__ void experts_tile(const EgArgs& p, const Routing& r, 
         info[threadIdx.x].at = (int)threadIdx.x < rows.count && pair >= 0 ? (int64_t)pair * p.n : -1;
     }
     auto issue_lhs = [&](int chunk, int buf) __attribute__((always_inline)) {
-        const int64_t at = (int64_t)min(chunk, last_chunk) * (64 * kPer);
+        const int64_t at = (int64_t)min(chunk, last_chunk) * (32 * kSteps * kPer);
 #pragma unroll
         for (int j = 0; j < kLoads; j++) load16_to_lds(src[j] + at, (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds0 + buf * L::kChunk + (first + j) * 1024)));
     };
@@ -119,7 +124,7 @@ __device__ __forceinline__ void experts_tile(const EgArgs& p, const Routing& r, 
         if constexpr (kHasSums) load16_to_lds(sums_src + (int64_t)unit * 32, (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds0 + L::kS + (buf * FM + sums_tile) * 1024)));
     };
 
-    float16v T[FM], P[FM], U[kUnit ? FM : 1];
+    float16v T[FM], P[FM], M, U[kUnit ? FM : 1];
 #pragma unroll
     for (int a = 0; a < FM; a++)
 #pragma unroll
@@ -128,16 +133,16 @@ __device__ __forceinline__ void experts_tile(const EgArgs& p, const Routing& r, 
             if constexpr (kUnit) U[a][i] = 0.0f;
         }
     const float16v zero16 = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    // where a lane's operands of the two steps of a chunk lie
-    uint32_t at_step[2];
+    // where a lane's operands of the steps of a chunk lie
+    uint32_t at_step[kSteps];
 #pragma unroll
-    for (int t = 0; t < 2; t++) at_step[t] = row * 64 + (((2 * t + g) ^ ((row >> 2) & 3)) << 4);
+    for (int t = 0; t < kSteps; t++) at_step[t] = row * (32 * kSteps) + turned(2 * t + g, row) * 16;
     half8 af[2][FM][kPer], b[2][W::kPlanes];
     auto read_lhs = [&](int step, int slot, uint32_t base) __attribute__((always_inline)) {
 #pragma unroll
         for (int a = 0; a < FM; a++)
 #pragma unroll
-            for (int q = 0; q < kPer; q++) af[slot][a][q] = *(const half8*)(smem + base + at_step[step] + (q * FM + a) * 2048);
+            for (int q = 0; q < kPer; q++) af[slot][a][q] = *(const half8*)(smem + base + at_step[step] + (q * FM + a) * (1024 * kSteps));
     };
 
     // (From here on the loads are counted: an ordinary one among them would wait for all.)
@@ -170,24 +175,24 @@ __device__ __forceinline__ void experts_tile(const EgArgs& p, const Routing& r, 
         }
         __builtin_amdgcn_sched_barrier(0);
         unrolled<16>([&](auto tt) __attribute__((always_inline)) {
-            constexpr int t = decltype(tt)::value, cur = t & 1, entered = t / 2 + 1;
-            if constexpr (t % 2 == 1) {
+            constexpr int t = decltype(tt)::value, cur = t & 1, entered = t / kSteps + 1;
+            if constexpr (t % kSteps == kSteps - 1) {
                 // The next chunk has arrived (asked for kBufs - 1 boundaries ago; younger: the chunks after it, and the next unit's weights and sums where they were asked for since), and every wavefront has
                 // read this one's operands into registers: its buffer takes the chunk after those that are there.  At a unit's end the weights are older than the chunk.
-                static_assert(kBufs - 1 < kEgChunks, "the weights of the next unit are older than its first chunk");
+                static_assert(kBufs - 1 < kChunks, "the weights of the next unit are older than its first chunk");
                 wait_vmcnt<(kBufs - 2) * kLoads + (entered <= kBufs - 1 ? kAhead : 0)>();
                 __syncthreads();
-                issue_lhs(u * kEgChunks + entered + kBufs - 1, buf);
+                issue_lhs(u * kChunks + entered + kBufs - 1, buf);
                 buf = buf == kBufs - 1 ? 0 : buf + 1;
             }
-            read_lhs((t + 1) % 2, cur ^ 1, (uint32_t)(buf * L::kChunk));
+            read_lhs((t + 1) % kSteps, cur ^ 1, (uint32_t)(buf * L::kChunk));
             if constexpr (W::kAsync) {
                 if constexpr (t + 1 == 16) w.open(next, (u + 1) & 1);
             }
             w.template before_step<t>();
             // one row tile every three steps, the last at steps 14 and 15
             constexpr int min_a = (t - 14 + 3 * (FM - 1)) / 3, min_at = 14 - 3 * (FM - 1);
-            constexpr bool min_now = W::kMin && t >= min_at && (t - min_at) % 3 == 0;
+            constexpr bool min_now = W::kMin && t >= min_at && (t - min_at) % 3 == 0, min_add = W::kMin && t > min_at && (t - min_at) % 3 == 1;
             half8 sf;
             if constexpr (min_now) sf = *(const half8*)(smem + L::kS + ((u & 1) * FM + min_a) * 1024 + lane * 16);
             if constexpr (W::kMin && HILO && t < 5) {
@@ -241,7 +246,6 @@ __device__ __forceinline__ void experts_tile(const EgArgs& p, const Routing& r, 
 #pragma unroll
                         for (int a = 0; a < FM; a++) P[a] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af[cur][a][q], b[cur][pl], P[a], 0, 0, 0);
             }
-            float16v M;
             if constexpr (min_now) {
                 if constexpr (HILO) {
                     M = __builtin_amdgcn_mfma_f32_32x32x16_f16(sf, w.offsets_lo(), zero16, 0, 0, 0);
@@ -249,6 +253,8 @@ __device__ __forceinline__ void experts_tile(const EgArgs& p, const Routing& r, 
                 } else {
                     M = __builtin_amdgcn_mfma_f32_32x32x16_f16(sf, w.min_operand(0), zero16, 0, 0, 0);
                 }
+            }
+            if constexpr (min_add) {  // (a step later: the product takes its time)
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     if constexpr (kUnit) U[min_a][i] = dmin * M[i];
@@ -260,7 +266,7 @@ __device__ __forceinline__ void experts_tile(const EgArgs& p, const Routing& r, 
             }
             w.template step<(t + 1) % 16>(0, b[cur ^ 1]);
             if constexpr (!W::kQ8 && t != 0) {
-                constexpr int kMfma = FM * kPer * W::kPlanes, kValu = (W::kPlanes == 2 ? 28 : 12) + (min_now ? 16 : 0);  // spread evenly
+                constexpr int kMfma = FM * kPer * W::kPlanes, kValu = (W::kPlanes == 2 ? 28 : 12) + (min_add ? 16 : 0);  // spread evenly
                 unrolled<kMfma + (min_now ? (HILO ? 2 : 1) : 0)>([&](auto) __attribute__((always_inline)) {
                     __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
                     __builtin_amdgcn_sched_group_barrier(0x2, (kValu + kMfma - 1) / kMfma, 0);
@@ -334,11 +340,17 @@ __device__ __forceinline__ void zero_tile(const EgArgs& p, const Routing& r, con
 
 template <int ENC, int FM, bool HILO, bool GATED>
 __global__ __launch_bounds__(64 * kEgWaves, 2) void experts_gemm_kernel(EgArgs p, Routing r) {
-    const ExpertRows rows = uniform(find_rows<32 * FM>(r, (int)blockIdx.y, threadIdx.x & 63));
+    // The tiles, those of one group of rows after the other, in eight equal parts: one for each XCD (ids congruent mod 8), in whose L2 an expert's weights and rows then are, once.
+    const uint32_t cols = (uint32_t)(p.n + (GATED ? 63 : 127)) / (GATED ? 64 : 128);
+    int col_tile = 0;
+    const ExpertRows rows = uniform(find_rows_of<32 * FM>(r, threadIdx.x & 63, [&](int groups) {
+        const int64_t tiles = (int64_t)groups * cols, place = (tiles * blockIdx.x >> 3) + blockIdx.y + (int64_t)blockIdx.z * gridDim.y;
+        if (place >= tiles * (blockIdx.x + 1) >> 3) return -1;
+        const int group = (int)((uint32_t)place / cols);
+        col_tile = __builtin_amdgcn_readfirstlane((int)((uint32_t)place - (uint32_t)group * cols));
+        return group;
+    }));
     if (rows.count == 0) return;
-    // columns of one expert go over the XCDs, beginning with another one for each
-    const int col_tile = (int)blockIdx.z * 8 + (((int)blockIdx.x + rows.expert) & 7);
-    if (col_tile * (GATED ? 64 : 128) >= p.n) return;
     if (rows.expert >= r.experts) return zero_tile<GATED>(p, r, rows, col_tile);
     if constexpr (FM > 2) {
         if (rows.count > 64) return experts_tile<ENC, 4, HILO, GATED>(p, r, rows, col_tile);
@@ -354,7 +366,7 @@ __global__ __launch_bounds__(64 * kEgWaves, 2) void experts_gemm_kernel(EgArgs p
 // ---------------------------------------------------------------------------------------------------------------------------
 // A row by TPR threads, eight columns a thread and turn.
 template <typename AT, int TPR>
-__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void experts_prep_kernel(const AT* __restrict__ a, int64_t rows, int k, int units, int with_sums, uint8_t* __restrict__ a16,
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void experts_prep_kernel(const AT* __restrict__ a, int64_t rows, int k, int units, int with_sums, int chunk_log, uint8_t* __restrict__ a16,
                                                                              uint8_t* __restrict__ sums, float* __restrict__ inv) {
     constexpr bool kF32 = sizeof(AT) == 4;
     constexpr int kThreads = TPR > 256 ? TPR : 256, kPer = kF32 ? 2 : 1, kHeld = 4;
@@ -397,9 +409,9 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void experts_prep_kernel(con
     auto emit = [&](int pc, const LhsPiece<AT>& x) __attribute__((always_inline)) {
         float v[8];
         unpack_piece(x, v);
-        // columns 8 pc ..: chunk blk, half g, step a: piece 2 a + g
-        const int blk = pc >> 2, at_g = (pc >> 1) & 1;
-        uint8_t* const at = to + blk * (64 * kPer) + (2 * (pc & 1) + at_g) * 16;
+        // columns 8 pc ..: block blk of 32, half g, step 2 blk + a: piece 2 (step within the chunk) + g
+        const int blk = pc >> 2, at_g = (pc >> 1) & 1, step = 2 * blk + (pc & 1), plane = 32 << chunk_log;
+        uint8_t* const at = to + (step >> chunk_log) * (plane * kPer) + (2 * (step & ((1 << chunk_log) - 1)) + at_g) * 16;
         constexpr int perm[8] = {0, 2, 1, 3, 4, 6, 5, 7};
 #pragma unroll
         for (int i = 0; i < 8; i++) v[i] *= s;
@@ -417,7 +429,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void experts_prep_kernel(con
             }
 #pragma unroll
             for (int i = 0; i < 4; i++) lo.u[i] = narrow2(rest[2 * i], rest[2 * i + 1]);
-            *(half8*)(at + 64) = lo.h;
+            *(half8*)(at + plane) = lo.h;
         }
         if (with_sums) {
             float sum = 0.0f;
@@ -449,7 +461,8 @@ __global__ __launch_bounds__(256) void experts_prep_q8_kernel(const AT* __restri
     if (row >= rows) return;  // (whole blocks: a multiple of four threads)
     const int pc = (int)(i - row * (units * 32)), pieces = k >> 3;
     if (pc == 0) inv[row] = 1.0f;
-    const int blk = pc >> 2, sub = pc & 3, g = sub & 1;  // columns 32 blk + 16 a + 8 g: step a of chunk blk
+    constexpr int kSteps = eg_steps(QMM_Q4_0);
+    const int blk = pc >> 2, sub = pc & 3, g = sub & 1, step = 2 * blk + (sub >> 1);  // columns 32 blk + 16 a + 8 g: step 2 blk + a
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (pc < pieces) unpack_piece(load_piece(a + row * k + pc * 8), v);
     float mx = 0.0f;
@@ -463,7 +476,7 @@ __global__ __launch_bounds__(256) void experts_prep_q8_kernel(const AT* __restri
     gd_u4 o;
 #pragma unroll
     for (int j = 0; j < 4; j++) o[j] = pack_half2((float)q8_0_code(v[perm[2 * j]], id), (float)q8_0_code(v[perm[2 * j + 1]], id));
-    *(gd_u4*)(a16 + row * units * 512 + blk * 64 + (2 * (sub >> 1) + g) * 16) = o;
+    *(gd_u4*)(a16 + row * units * 512 + (step / kSteps) * (32 * kSteps) + (2 * (step % kSteps) + g) * 16) = o;
     if (sub == 0) {
         uint16_t* const sp = (uint16_t*)(sums + (row * units + (blk >> 3)) * 32) + (blk & 7);
         sp[0] = dh;
@@ -493,21 +506,23 @@ hipError_t run_prep(const ExpertCall& c, const EgArgs& p, hipStream_t s) {
     if (c.encoding == QMM_Q4_0) {
         experts_prep_q8_kernel<AT><<<dim3((unsigned)((c.lhs_rows * p.units * 32 + 255) / 256)), dim3(256), 0, s>>>(a, c.lhs_rows, k, p.units, a16, sums, inv);
     } else {
-        const int with_sums = c.encoding != QMM_Q6_K;
-        if (k <= 1024) experts_prep_kernel<AT, 64><<<dim3((unsigned)((c.lhs_rows + 3) / 4)), dim3(256), 0, s>>>(a, c.lhs_rows, k, p.units, with_sums, a16, sums, inv);
-        else if (k <= 8192) experts_prep_kernel<AT, 256><<<dim3((unsigned)c.lhs_rows), dim3(256), 0, s>>>(a, c.lhs_rows, k, p.units, with_sums, a16, sums, inv);
-        else experts_prep_kernel<AT, 1024><<<dim3((unsigned)c.lhs_rows), dim3(1024), 0, s>>>(a, c.lhs_rows, k, p.units, with_sums, a16, sums, inv);
+        const int with_sums = c.encoding != QMM_Q6_K, chunk_log = eg_steps(c.encoding) == 4 ? 2 : 1;
+        if (k <= 1024) experts_prep_kernel<AT, 64><<<dim3((unsigned)((c.lhs_rows + 3) / 4)), dim3(256), 0, s>>>(a, c.lhs_rows, k, p.units, with_sums, chunk_log, a16, sums, inv);
+        else if (k <= 8192) experts_prep_kernel<AT, 256><<<dim3((unsigned)c.lhs_rows), dim3(256), 0, s>>>(a, c.lhs_rows, k, p.units, with_sums, chunk_log, a16, sums, inv);
+        else experts_prep_kernel<AT, 1024><<<dim3((unsigned)c.lhs_rows), dim3(1024), 0, s>>>(a, c.lhs_rows, k, p.units, with_sums, chunk_log, a16, sums, inv);
     }
     return hipGetLastError();
 }
+
+int64_t eg_tiles(const Routing& r, int fm, int64_t n, bool gated) { return most_groups(r.pairs, r.experts, 32 * fm) * ((n + (gated ? 63 : 127)) / (gated ? 64 : 128)); }
 
 template <int ENC, int FM, bool HILO, bool GATED>
 hipError_t run_gemm(const EgArgs& p, const Routing& r, hipStream_t s) {
     constexpr int lds = std::max(std::max(EgLds<ENC, FM, HILO>::kBytes, EgLds<ENC, 1, HILO>::kBytes), EgLds<ENC, std::min(FM, 2), HILO>::kBytes);
     const hipError_t e = allow_full_lds<experts_gemm_kernel<ENC, FM, HILO, GATED>>();
     if (e != hipSuccess) return e;
-    const int cols = GATED ? 64 : 128;
-    experts_gemm_kernel<ENC, FM, HILO, GATED><<<dim3(8, (unsigned)most_groups(r.pairs, r.experts, 32 * FM), (unsigned)((p.n + 8 * cols - 1) / (8 * cols))), dim3(64 * kEgWaves), lds, s>>>(p, r);
+    const int64_t tiles = eg_tiles(r, FM, p.n, GATED), part = (tiles + 7) / 8, y = std::min<int64_t>(part, 32768);
+    experts_gemm_kernel<ENC, FM, HILO, GATED><<<dim3(8, (unsigned)y, (unsigned)((part + y - 1) / y)), dim3(64 * kEgWaves), lds, s>>>(p, r);
     return hipGetLastError();
 }
 template <int ENC, int FM, bool HILO>
@@ -540,7 +555,7 @@ bool experts_gemm_supported(const ExpertCall& c, const Routing& r) {
     if (kernel_disabled("experts_gemm")) return false;
     const int64_t bpb = c.encoding == QMM_Q4_0 ? Q4_0_BPB : c.encoding == QMM_Q4_K ? Q4_K_BPB : c.encoding == QMM_Q5_K ? Q5_K_BPB : Q6_K_BPB, epb = c.encoding == QMM_Q4_0 ? 32 : 256;
     const int64_t blocks = c.n * (c.k / epb);
-    if (blocks * bpb > 0x7fffffff || most_groups(r.pairs, r.experts, 64) > 65535) return false;  // (offsets in a matrix have 32 bits)
+    if (blocks * bpb > 0x7fffffff || eg_tiles(r, eg_rows(c, r), c.n, c.gated) > 0x7fffffff) return false;  // (offsets in a matrix, and the tiles' numbers, have 32 bits)
     const uintptr_t all = (uintptr_t)c.w[0] | (uintptr_t)c.expert_stride[0] | (c.gated ? (uintptr_t)c.w[1] | (uintptr_t)c.expert_stride[1] : 0);
     if (c.encoding == QMM_Q4_0) return (all & 1) == 0;
     if (all & 3) return false;

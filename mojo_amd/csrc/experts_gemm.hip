@@ -62,7 +62,8 @@ struct EgLds {
     static constexpr int kPer = HILO ? 2 : 1, kSteps = eg_steps(ENC), kChunk = FM * 1024 * kSteps * kPer, kWeights = kEgWaves * W::kBufs * W::kStage, kSums = W::kMin || W::kQ8 ? 2 * FM * 1024 : 0;
     static constexpr int kResultRow = 40, kResults = kEgWaves * 32 * std::min(FM, 2) * kResultRow * 4, kInfoBytes = 32 * FM * (int)sizeof(EgRow);
     static constexpr int bytes(int bufs) { return std::max(bufs * kChunk + kWeights + kSums, kResults) + kInfoBytes; }
-    static constexpr int kBufs = bytes(4) <= kLdsPerCu / 2 ? 4 : bytes(3) <= kLdsPerCu / 2 ? 3 : 2;
+    static constexpr int kShare = kLdsPerCu / (FM == 1 && bytes(2) <= kLdsPerCu / 3 ? 3 : 2);
+    static constexpr int kBufs = bytes(4) <= kShare ? 4 : bytes(3) <= kShare ? 3 : 2;
     static constexpr int kW = kBufs * kChunk, kS = kW + kWeights, kInfo = std::max(kS + kSums, kResults), kBytes = bytes(kBufs);
     static_assert(kBytes <= kLdsPerCu / 2, "two on a compute unit");
 };
@@ -543,10 +544,14 @@ hipError_t run_gemm(const EgArgs& p, const Routing& r, int fm, bool hilo, hipStr
     return run_gemm_rows<ENC, false>(p, r, fm, s);
 }
 
-// Rows of a group, in 32s: as many as an expert has on average, up to what the registers hold.
+// Rows of a group, in 32s, by what an expert has on average.  Few rows: more groups fill the part better, and less is computed for rows that are not there; many: a weight is unpacked once for more of them.
+// us with 32 / 64 / 128 rows, bf16 rows, 8 of 64 experts, 1024 x 2048: Q4_K 32 rows an expert 37 / 44 / 42, 64 56 / 55 / 56, 128 88 / 81 / 85, 192 120 / 104 / 105; Q6_K (two products a weight) 24 60 / 62 / 56,
+// 48 85 / 65 / 74, 128 160 / 120 / 118, 192 211 / 151 / 145; 2 of 8, 14336 x 4096: Q4_K 32 106 / 103 / 103, 64 171 / 157 / 155, 256 498 / 390 / 344; Q4_0 (no 128) 64 68 / 74, 96 96 / 87; fp32 rows Q4_K 48 69 / 73, 96 111 / 104.
 int eg_rows(const ExpertCall& c, const Routing& r) {
     const int64_t mean = r.pairs / r.experts;
-    return std::min(mean <= 32 ? 1 : mean <= 64 ? 2 : 4, eg_most(c.encoding, c.lhs_dtype == QMM_F32));
+    const bool f32 = c.lhs_dtype == QMM_F32;
+    const int one = c.encoding == QMM_Q4_0 ? 80 : !f32 && (c.encoding == QMM_Q5_K || c.encoding == QMM_Q6_K) ? 24 : 48;
+    return std::min(mean <= one ? 1 : mean <= 160 ? 2 : 4, eg_most(c.encoding, f32));
 }
 
 }  // namespace

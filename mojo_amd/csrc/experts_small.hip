@@ -24,14 +24,15 @@ struct EsPlan {
     int waves, groups, per, grid, chunk;
     size_t lds;
 };
-// tiles: of one group of rows; groups_y: groups of rows; nblk: super-blocks that a workgroup walks
+// tiles: of one group of rows; groups_y: groups of rows that are expected; nblk: super-blocks that a workgroup walks.  One round of workgroups if there are as many groups as expected, but no more than 16 tiles
+// each: a group more than expected would otherwise be a round more (2 of 8 experts, 14336 x 4096 Q4_K, 16 fp32 rows 65 us, without the bound 46 or 90, with 8 tiles 71).
 EsPlan es_plan(int encoding, int mrows, int64_t tiles, int64_t groups_y, int64_t nblk) {
     EsPlan p;
     p.groups = (int)((nblk + kSmallWaves - 1) / kSmallWaves);
     p.waves = (int)((nblk + p.groups - 1) / p.groups);
     const int per_cu = std::max(1, kSmallWaves / p.waves);
     const int64_t places = std::max<int64_t>(1, (int64_t)compute_units() * per_cu / groups_y);
-    p.per = (int)((tiles + places - 1) / places);
+    p.per = (int)std::min<int64_t>((tiles + places - 1) / places, 16);
     p.grid = (int)((tiles + p.per - 1) / p.per);
     const int slot = encoding == QMM_Q4_0 || encoding == QMM_Q4_K ? SmallItem<QMM_Q4_K>::kSlot : encoding == QMM_Q5_K ? SmallItem<QMM_Q5_K>::kSlot : SmallItem<QMM_Q6_K>::kSlot;
     const int lr = mrows <= 4 ? 1 : mrows / 4, ring = p.waves * 2 * slot, bytes = (p.waves + (p.groups > 1 ? 1 : 0)) * lr * 256;
@@ -63,16 +64,19 @@ hipError_t run_small(const ExpertCall& c, const SmallExperts& ex, int64_t groups
                    : run_small<ENC, MROWS, AT, kSmallPlain, kSmallByExpert>(c, ex, groups_y, expected, out, out_bf16, s);
 }
 
-// Rows of a group: what an expert that has any gets, on average over those (each token's experts are others).
+// Experts that get a row, if none is preferred, and the rows that each of them gets, on average.
+double es_with(const Routing& r) { return std::max(1.0, r.experts * (1.0 - pow(1.0 - std::min(1.0, (double)r.top / r.experts), (double)(r.pairs / r.top)))); }
+double es_mean(const Routing& r) { return r.pairs / es_with(r); }
+// Rows of a group.  us with 4 / 8 rows, 8 of 64 experts, 1024 x 2048 Q4_K: 2.3 rows an expert 17.9 / 18.9, 3.2 25.6 / 19.9; with 8 / 16: 6 27.4 / 33.1, 8 34.0 / 33.2.
 int es_rows(const ExpertCall& c, const Routing& r, int64_t& expected) {
     const int64_t tokens = r.pairs / r.top, most = small_most_rows(c.lhs_dtype);
     if (tokens == 1) {
         expected = r.pairs;
         return 1;
     }
-    const double with = r.experts * (1.0 - pow(1.0 - (double)r.top / r.experts, (double)tokens)), mean = r.pairs / std::max(with, 1.0);
-    const int rows = tokens <= 4 || mean <= 2.5 ? 4 : mean <= 5.5 || most == 8 ? 8 : 16;
-    expected = std::max<int64_t>(1, (int64_t)(with * std::max(1.0, mean / rows)));
+    const double mean = es_mean(r);
+    const int rows = tokens <= 4 || mean <= 2.5 ? 4 : mean <= 6.5 || most == 8 ? 8 : 16;
+    expected = std::max<int64_t>(1, (int64_t)(es_with(r) * std::max(1.0, mean / rows)));
     return rows;
 }
 int64_t es_groups(const Routing& r, int rows) { return r.pairs == r.top ? r.pairs : most_groups(r.pairs, r.experts, rows); }
@@ -109,11 +113,13 @@ bool es_takes(const ExpertCall& c) {
 
 }  // namespace
 
+// Up to 8 rows an expert, or 12 where the GEMM unpacks more (bf16 rows but for Q4_K).  us, this kernel / the GEMM (with its preparation): 8 of 64 experts, 1024 x 2048, bf16 Q4_K 4 rows 19.8 / 28.0, 6 33.1 / 28.3,
+// 12 33.3 / 29.1; Q6_K 8 45.3 / 40.3, 12 45.5 / 57.2; Q5_K 8 35.5 / 36.9, 12 35.8 / 43.8; fp32 Q4_K 8 29.5 / 31.3, 12 44.6 / 32.1; 2 of 8, 14336 x 4096, bf16 Q4_K 8 74 / 79, 12 105 / 88; Q6_K 12 112 / 136, 16 155 / 137.
 bool experts_small_wanted(const ExpertCall& c, const Routing& r) {
-    if (!es_takes(c)) return false;
+    if (!es_takes(c) || es_mean(r) > (c.lhs_dtype == QMM_F32 || c.encoding == QMM_Q4_K ? 8.0 : 12.0)) return false;
     int64_t expected;
     const int rows = es_rows(c, r, expected);
-    return r.pairs <= 4096 && es_groups(r, rows) <= 65535 && r.pairs <= (int64_t)r.experts * small_most_rows(c.lhs_dtype);
+    return es_groups(r, rows) <= 65535;
 }
 
 hipError_t launch_experts_small(const ExpertCall& c, const Routing& r, void* out, bool out_bf16, hipStream_t s) {

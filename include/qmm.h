@@ -308,7 +308,8 @@ typedef struct qmm_routing {
 } qmm_routing;
 
 /*
- * Matrix products grouped by expert: y[p, n] = lhs[row of p] . dequant(rhs[expert of p])^T with the products of qmm_matmul (Q4_0: the lhs quantised to Q8_0).
+ * Matrix products grouped by expert: y[p, n] = lhs[row of p] . dequant(rhs[expert of p])^T with the products of qmm_matmul (Q4_0: the lhs quantised to Q8_0 blocks,
+ * whose scale here is the largest magnitude times 1 / 127 where qmm_matmul divides by 127: another last bit now and then, and then perhaps a neighbouring code).
  *   QMM_EXPERTS_EACH    out[p, n] = y
  *   QMM_EXPERTS_SWIGLU  out[p, n] = silu(y of rhs) * (y of rhs2)
  *   QMM_EXPERTS_SUM     out[t, n] = residual[t, n] + sum over j of weights[top t + j] y[top t + j, n], in that order (residual: null, fp32 or bf16[tokens, n])

@@ -472,7 +472,7 @@ __global__ __launch_bounds__(256) void experts_prep_q8_kernel(const AT* __restri
     mx = fmaxf(mx, dpp_move<0xB1>(mx));
     mx = fmaxf(mx, dpp_move<0x4E>(mx));
     uint16_t dh;
-    const float id = q8_0_block_rule(mx, dh);
+    const float id = q8_0_block_rule<true>(mx, dh);
     constexpr int perm[8] = {0, 2, 1, 3, 4, 6, 5, 7};
     gd_u4 o;
 #pragma unroll

@@ -1,7 +1,7 @@
 // The experts' products for every shape: one wavefront takes one weight row (gated: one of gate and the same of up) of one expert for up to four of the expert's rows, a value at a time on the vector units.
 //
 // What the matrix-core kernels do not take goes here: weights at odd addresses, Q6_K rows with an odd number of blocks.  What bounds it is the unpacking, some twenty instructions a weight.
-// Q4_0: the lhs as Q8_0 codes and block scales (fp16, held as fp32), made by a launch in front; integer block dots, summed as qmatmul does.
+// Q4_0: the lhs as Q8_0 codes and block scales (fp16, held as fp32), made by a launch in front; integer block dots.
 // Also here: the weighted sum over the experts of a token, which ends the products of every kernel that leaves the pairs' results apart.
 #include <algorithm>
 
@@ -97,6 +97,22 @@ __global__ __launch_bounds__(64 * kErWaves) void experts_rows_kernel(ErArgs a, R
     }
 }
 
+// The lhs of Q4_0: codes and block scales, 32 lanes a block.
+template <typename AT>
+__global__ __launch_bounds__(256) void experts_quantize_kernel(const AT* __restrict__ x, int64_t blocks, int8_t* __restrict__ codes, float* __restrict__ dscale) {
+    const int64_t block = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5;
+    if (block >= blocks) return;
+    const int i = threadIdx.x & 31;
+    const float v = load_f32(x, block * 32 + i);
+    float amax = fabsf(v);
+#pragma unroll
+    for (int mask = 16; mask; mask >>= 1) amax = fmaxf(amax, __shfl_xor(amax, mask, 32));
+    uint16_t dh;
+    const float id = q8_0_block_rule<true>(amax, dh);
+    codes[block * 32 + i] = (int8_t)q8_0_code(v, id);
+    if (i == 0) dscale[block] = h2f(dh);
+}
+
 // Four results a thread (n a multiple of four, aligned rows) or one.
 template <int V>
 __global__ __launch_bounds__(256) void experts_combine_kernel(Routing r, const float* __restrict__ y, int n, const void* __restrict__ residual, int residual_bf16, void* __restrict__ out, int out_bf16) {
@@ -132,8 +148,8 @@ __global__ __launch_bounds__(256) void experts_combine_kernel(Routing r, const f
 
 }  // namespace
 
-// Q4_0: codes, then block scales and sums of codes (which nothing here reads)
-int64_t experts_rows_workspace_bytes(const ExpertCall& c) { return c.encoding == QMM_Q4_0 ? (c.lhs_rows * c.k + 255) / 256 * 256 + c.lhs_rows * (c.k / 32) * 8 : 0; }
+// Q4_0: codes, then block scales
+int64_t experts_rows_workspace_bytes(const ExpertCall& c) { return c.encoding == QMM_Q4_0 ? (c.lhs_rows * c.k + 255) / 256 * 256 + c.lhs_rows * (c.k / 32) * 4 : 0; }
 
 hipError_t launch_experts_rows(const ExpertCall& c, const Routing& r, void* out, bool out_bf16, void* workspace, hipStream_t s) {
     ErArgs a{c.lhs, c.lhs_top, nullptr, {c.w[0], c.w[1]}, {c.expert_stride[0], c.expert_stride[1]}, 0, c.gated, (int)c.n, (int)c.k, out, out_bf16};
@@ -141,7 +157,10 @@ hipError_t launch_experts_rows(const ExpertCall& c, const Routing& r, void* out,
     if (c.encoding == QMM_Q4_0) {
         int8_t* const codes = (int8_t*)workspace;
         float* const dscale = (float*)(codes + (c.lhs_rows * c.k + 255) / 256 * 256);
-        const hipError_t e = launch_quantize_q8_0(c.lhs, c.lhs_dtype, c.lhs_rows, c.k, nullptr, codes, dscale, dscale + c.lhs_rows * (c.k / 32), s);
+        const int64_t blocks = c.lhs_rows * (c.k / 32);
+        if (c.lhs_dtype == QMM_F32) experts_quantize_kernel<<<dim3((unsigned)((blocks + 7) / 8)), dim3(256), 0, s>>>((const float*)c.lhs, blocks, codes, dscale);
+        else experts_quantize_kernel<<<dim3((unsigned)((blocks + 7) / 8)), dim3(256), 0, s>>>((const uint16_t*)c.lhs, blocks, codes, dscale);
+        const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
         a.lhs = codes;
         a.dscale = dscale;

@@ -209,7 +209,7 @@ __device__ __forceinline__ void small_body(const MmMats& mats, const AT* __restr
         if constexpr (kQ8) {
 #pragma unroll
             for (int r0 = 0; r0 < MROWS; r0 += kPass) {
-                small_quantize<kPass>(xr, r0, area, lane);
+                small_quantize<kPass, EX != kSmallNoExperts>(xr, r0, area, lane);
                 asm volatile("" ::: "memory");  // (scales are written as 16-bit numbers and read as vectors: not to be reordered)
                 __builtin_amdgcn_wave_barrier();
                 if ((nn & 3) < RN && my_row >= r0 && my_row < r0 + kPass) {

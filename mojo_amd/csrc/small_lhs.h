@@ -164,7 +164,7 @@ constexpr int kSmallCodes = 272;  // an lhs row of 256 columns as Q8_0: codes, b
 
 // Rows r0 .. r0 + PASS - 1 (at most four) as Q8_0 to `area`, kSmallCodes bytes each.  The 32 codes of a block in eight dwords: columns 4 i .. 4 i + 3 and 16 + 4 i .. + 3 lie in dwords 2 i and 2 i + 1.
 // Eight lanes hold a block of every row; the divisions of a block's rule are made once for four rows, by the lane whose number is the row's.
-template <int PASS, typename RAW, int ROWS>
+template <int PASS, bool TIMES = false, typename RAW, int ROWS>
 __device__ __forceinline__ void small_quantize(const RAW (&xr)[ROWS], int r0, uint8_t* area, int lane) {
     static_assert(PASS <= 4, "a lane of four for each row");
     float x[PASS][4], amax[PASS];
@@ -187,7 +187,7 @@ __device__ __forceinline__ void small_quantize(const RAW (&xr)[ROWS], int r0, ui
 #pragma unroll
     for (int j = 1; j < PASS; j++) top = mine == j ? amax[j] : top;
     uint16_t dh;
-    const float id = q8_0_block_rule(top, dh);
+    const float id = q8_0_block_rule<TIMES>(top, dh);
     __builtin_amdgcn_wave_barrier();
     if ((lane & 4) == 0 && mine < PASS) *(uint16_t*)(area + mine * kSmallCodes + 256 + 2 * (lane >> 3)) = dh;
 #pragma unroll

@@ -218,7 +218,7 @@ def qmatmul_experts(encoding: QuantizationEncoding, lhs: torch.Tensor, rhs: torc
 
     ``rhs`` is ``uint8[experts, N, K / epb * bpb]`` (the matrix of an expert contiguous, the experts at any distance: a slice of a tensor that holds more).  ``lhs``
     is float32 or bfloat16 ``[..., K]``, a row for each token or one for each of its experts (``[..., top, K]``).  The products are those of :func:`qmatmul` on
-    each expert's rows.
+    each expert's rows (Q4_0: of the lhs in Q8_0 blocks, whose scale is the largest magnitude times ``1 / 127`` where :func:`qmatmul` divides by 127).
     """
     return _experts(_lib.QMM_EXPERTS_EACH, "qmatmul_experts", encoding, lhs, ((rhs, "rhs"),), routing, None, out_dtype)
 

@@ -26,12 +26,12 @@ def weights64(encoding, packed):
 
 
 def lhs64(encoding, x):
-    """The lhs as the products take it: Q4_0 rounds it to Q8_0 (fp32 rule, fp16 scale, halves away from zero)."""
+    """The lhs as the products take it: Q4_0 rounds it to Q8_0 (scale = largest times 1 / 127 in fp32, kept as fp16, codes with halves away from zero)."""
     x = x.float()
     if encoding != QE.Q4_0:
         return x.double()
     b = x.reshape(*x.shape[:-1], -1, 32)
-    d = b.abs().amax(-1, keepdim=True) / 127.0
+    d = b.abs().amax(-1, keepdim=True) * torch.tensor(np.float32(1) / np.float32(127))
     t = (b * torch.where(d != 0, 1.0 / d, torch.zeros_like(d))).double()
     codes = torch.sign(t) * torch.floor(t.abs() + 0.5)
     return (codes * d.half().double()).reshape(x.shape)

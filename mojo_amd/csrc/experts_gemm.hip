@@ -32,16 +32,126 @@ struct EgArgs {
     int out_bf16;
 };
 
-// The weights of one wavefront.  Loads to LDS (kAsync), a unit ahead, or through registers (Q4_0, rows of any number of blocks at any even address).
+// The weights of one wavefront: loads to LDS, a unit ahead.
 template <int ENC, bool CENTER>
 struct EgStaged : StagedOf<ENC, 16, CENTER> {
     using Base = StagedOf<ENC, 16, CENTER>;
-    static constexpr bool kAsync = true, kQ8 = false;
+    static constexpr bool kQ8 = false;
     static constexpr int kBufs = 2, kAhead = Base::kLoads;
+    __device__ __forceinline__ bool load_last(int) { return false; }
 };
-struct EgQ40 : Q40Weights<1> {
-    static constexpr bool kAsync = false, kQ8 = true;
-    static constexpr int kBufs = 1, kAhead = 0;
+// Q4_0: a row's eight blocks of a unit from the last multiple of four on, in nine pieces of 16 bytes and four bytes that only rows which begin two bytes later need.  The fields of a row lie `skew` (0 or 2)
+// bytes into its pieces.  Rows of any number of blocks: the unit that ends the row, where it is a partial one, is the first to be multiplied, comes through registers, and is zeros behind the row's end.  So the
+// loads to LDS never read beyond a row: a row with skew has an odd number of blocks and ends in a partial unit (or the matrices do not begin at multiples of four, see experts_gemm_supported).
+// Decoding as in Q40Weights: lane half g takes bytes 8 g .. 8 g + 7 of a block, low nibbles first.
+struct EgQ40 : NoOffsets {
+    static constexpr bool kQ8 = true, kMin = false;
+    static constexpr int kPlanes = 1, kBufs = 2, kUnit = 8 * Q4_0_BPB, kPieces = kUnit / 16, kTotal = 32 * kPieces, kWide = (kTotal + 63) / 64, kLoads = kWide + 1, kAhead = kLoads;
+    static constexpr int kTail = kTotal * 16, kStage = kTail + 128;
+    const uint8_t* w;
+    uint8_t* stage;
+    const uint8_t* cur;
+    const uint8_t* tail;
+    uint32_t stage_lds, off[kWide], off_tail, skew, mine;  // mine: where the lane's row (of 32) begins
+    int row_bytes, g, lane_;
+    uint32_t x[2][3];
+    uint32_t d[8], last;  // (of lanes g = 0; zero in the others)
+    uint32_t top0 = code_top(0x64006400u), top1 = code_top(0x54005400u);
+    struct __attribute__((packed, aligned(2))) Bytes16 {
+        gd_u4 v;
+    };
+    // from w on
+    __device__ __forceinline__ uint32_t row_at(const WeightTensors& t, int row) const { return (uint32_t)min(row, t.n - 1) * (uint32_t)row_bytes + ((uint32_t)(uintptr_t)t.w & 2u); }
+    __device__ __forceinline__ void init(const WeightTensors& t, int n0, int lane, uint8_t* at) {
+        g = lane >> 5;
+        lane_ = lane;
+        stage = at;
+        stage_lds = lds_address(at);
+        w = t.w - ((uintptr_t)t.w & 2);
+        row_bytes = t.k / 32 * Q4_0_BPB;
+        const int step = row_bytes < kUnit ? 0 : 16;  // (the only unit is partial: what is asked for in advance and never looked at stays within the row)
+#pragma unroll
+        for (int j = 0; j < kWide; j++) {
+            const int i = min(j * 64 + lane, kTotal - 1), row = i / kPieces;
+            off[j] = (row_at(t, n0 + row) & ~2u) + step * (i - row * kPieces);
+        }
+        mine = row_at(t, n0 + (lane & 31));
+        skew = mine & 2u;
+        off_tail = (mine & ~2u) + (skew && step ? kUnit : 0);
+    }
+    template <int J>
+    __device__ __forceinline__ void issue(int unit, int buf) {
+        const uint8_t* b = w + (int64_t)unit * kUnit;
+        const uint32_t to = stage_lds + buf * kStage;
+        if constexpr (J < kWide) {
+            if (J * 64 + 63 < kTotal || J * 64 + lane_ < kTotal) load16_to_lds(off[J], b, to + J * 1024);
+        } else if (lane_ < 32) {
+            load4_to_lds(b + off_tail, to + kTail);
+        }
+    }
+    // the partial unit at the rows' end, to the first buffer
+    __device__ __forceinline__ bool load_last(int unit) {
+        const int left = row_bytes - unit * kUnit;
+        if (left == kUnit) return false;
+#pragma unroll
+        for (int j = 0; j < kWide; j++) {
+            const int i = min(j * 64 + lane_, kTotal - 1), row = i / kPieces, piece = 16 * (i - row * kPieces);
+            const uint32_t begin = (uint32_t)__shfl((int)mine, row);
+            // the last 16 bytes of the row, moved down to the place the piece would have (rows are at least 18 bytes long)
+            const int over = max(piece + 16 - left - (int)(begin & 2u), 0);
+            const gd_u4 v = ((const Bytes16*)(w + (int64_t)unit * kUnit + (begin & ~2u) + piece - over))->v;
+            uint64_t lo = v.x | (uint64_t)v.y << 32, hi = v.z | (uint64_t)v.w << 32;
+            if (over >= 16) lo = hi = 0;
+            else if (over >= 8) { lo = hi >> (8 * over - 64); hi = 0; }
+            else if (over > 0) { lo = (lo >> (8 * over)) | (hi << (64 - 8 * over)); hi >>= 8 * over; }
+            if (j * 64 + 63 < kTotal || j * 64 + lane_ < kTotal) *(gd_u4*)(stage + j * 1024 + lane_ * 16) = gd_u4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+        }
+        return true;
+    }
+    // Block b begins with its scale at 18 b + skew of the row; the lane's eight code bytes are two bytes and 8 g further: from a multiple of four on, or two bytes behind one.
+    template <int B>
+    __device__ __forceinline__ void read_block() {
+        const uint32_t* const p = (const uint32_t*)(cur + 8 * g + (B & 1 ? 18 * B + 2 : 18 * B + 2 * skew));
+        x[B & 1][0] = p[0];
+        x[B & 1][1] = p[1];
+        x[B & 1][2] = B == 7 ? *(const uint32_t*)tail : p[2];
+    }
+    __device__ __forceinline__ void open(int, int buf) {
+        const uint8_t* const b = stage + buf * kStage;
+        cur = b + (lane_ & 31) * kUnit;
+        tail = g ? b + kTail + 4 * (lane_ & 31) : cur + 136;
+        read_block<0>();
+        last = d[7];  // (the block before the next unit's still has to be scaled)
+#pragma unroll
+        for (int i = 0; i < 8; i++) d[i] = g ? 0u : (uint32_t)*(const uint16_t*)(cur + skew + 18 * i);
+    }
+    template <int T>
+    __device__ __forceinline__ void step(int, half8 (&b)[1]) const {
+        constexpr int blk = T >> 1;
+        const uint32_t turn = blk & 1 ? skew : skew ^ 2u;
+        uint32_t v[4];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const uint32_t q = __builtin_amdgcn_alignbyte(x[blk & 1][i + 1], x[blk & 1][i], turn), y = q >> 8;
+            if constexpr ((T & 1) == 0) {
+                v[2 * i] = pk_add((q & 0x000F000Fu) | top0, 0xE408E408u);  // 1024 + q - 1032
+                v[2 * i + 1] = pk_add((y & 0x000F000Fu) | top0, 0xE408E408u);
+            } else {
+                v[2 * i] = pk_add((q & 0x00F000F0u) | top1, 0xD480D480u);  // 64 + q - 72
+                v[2 * i + 1] = pk_add((y & 0x00F000F0u) | top1, 0xD480D480u);
+            }
+        }
+        b[0] = pack4(v[0], v[1], v[2], v[3]);
+    }
+    template <int T>
+    __device__ __forceinline__ void before_step() {
+        if constexpr ((T & 1) == 0 && T < 14) read_block<(T >> 1) + 1>();
+    }
+    template <int B>
+    __device__ __forceinline__ half8 scale_operand(int) const {
+        const uint32_t v = (B == 7 ? last : d[B]) << (16 * (B & 1));
+        return pack4(B >> 1 == 0 ? v : 0u, B >> 1 == 1 ? v : 0u, B >> 1 == 2 ? v : 0u, B >> 1 == 3 ? v : 0u);
+    }
 };
 template <int ENC, bool CENTER>
 using EgWeights = std::conditional_t<ENC == QMM_Q4_0, EgQ40, EgStaged<ENC == QMM_Q4_0 ? QMM_Q4_K : ENC, CENTER>>;
@@ -88,12 +198,12 @@ __device__ __forceinline__ void experts_tile(const EgArgs& p, const Routing& r, 
     EgRow* const info = (EgRow*)(smem + L::kInfo);
     WeightTensors wt{p.w[mat] + rows.expert * p.stride[mat], nullptr, nullptr, p.n, p.k, 0};
     const int units = p.units, last_chunk = units * kChunks - 1;
+    auto unit_at = [&](int u) __attribute__((always_inline)) { return !W::kQ8 ? u : u == 0 ? units - 1 : u - 1; };  // Q4_0: the last unit first
     const uint32_t lds0 = lds_address(smem);
     W w;
     w.init(wt, n0, lane, smem + L::kW + wave * W::kBufs * W::kStage);
     auto issue_weights = [&](int unit, int buf) __attribute__((always_inline)) {
-        if constexpr (W::kAsync) unrolled<W::kAhead>([&](auto j) __attribute__((always_inline)) { w.template issue<decltype(j)::value>(unit, buf); });
-        else w.load(unit);
+        unrolled<W::kAhead>([&](auto j) __attribute__((always_inline)) { w.template issue<decltype(j)::value>(unit, buf); });
     };
     auto lhs_row = [&](int i) __attribute__((always_inline)) { return max(pair_at(r, rows.first + min(i, rows.count - 1)), 0) / p.lhs_top; };
     // a row of a chunk is kPieces of 16 bytes; a piece's place is turned by the row, so that the same piece of 16 rows lies in all banks
@@ -117,7 +227,8 @@ __device__ __forceinline__ void experts_tile(const EgArgs& p, const Routing& r, 
         info[threadIdx.x].at = (int)threadIdx.x < rows.count && pair >= 0 ? (int64_t)pair * p.n : -1;
     }
     auto issue_lhs = [&](int chunk, int buf) __attribute__((always_inline)) {
-        const int64_t at = (int64_t)min(chunk, last_chunk) * (32 * kSteps * kPer);
+        const int c = min(chunk, last_chunk);
+        const int64_t at = (int64_t)(!W::kQ8 ? c : c < kChunks ? c + last_chunk + 1 - kChunks : c - kChunks) * (32 * kSteps * kPer);
 #pragma unroll
         for (int j = 0; j < kLoads; j++) load16_to_lds(src[j] + at, (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds0 + buf * L::kChunk + (first + j) * 1024)));
     };
@@ -147,21 +258,20 @@ __device__ __forceinline__ void experts_tile(const EgArgs& p, const Routing& r, 
     };
 
     // (From here on the loads are counted: an ordinary one among them would wait for all.)
-    issue_weights(0, 0);
-    issue_sums(0, 0);
+    if (!w.load_last(unit_at(0))) issue_weights(unit_at(0), 0);
+    issue_sums(unit_at(0), 0);
 #pragma unroll
     for (int c = 0; c < kBufs - 1; c++) issue_lhs(c, c);
     wait_vmcnt<(kBufs - 2) * kLoads>();
     __syncthreads();
     issue_lhs(kBufs - 1, kBufs - 1);
-    if constexpr (W::kAsync) w.open(0, 0);
-    else w.open();
+    w.open(unit_at(0), 0);
     read_lhs(0, 0, 0);
     w.template step<0>(0, b[0]);
     float d = 0.0f;
     int buf = 0;  // of the current chunk
     for (int u = 0; u < units; u++) {
-        const int next = min(u + 1, units - 1);
+        const int next = unit_at(min(u + 1, units - 1));
         // (nobody reads the sums and weights of the unit before any more)
         issue_weights(next, (u + 1) & 1);
         issue_sums(next, (u + 1) & 1);
@@ -187,9 +297,7 @@ __device__ __forceinline__ void experts_tile(const EgArgs& p, const Routing& r, 
                 buf = buf == kBufs - 1 ? 0 : buf + 1;
             }
             read_lhs((t + 1) % kSteps, cur ^ 1, (uint32_t)(buf * L::kChunk));
-            if constexpr (W::kAsync) {
-                if constexpr (t + 1 == 16) w.open(next, (u + 1) & 1);
-            }
+            if constexpr (t + 1 == 16) w.open(next, (u + 1) & 1);
             w.template before_step<t>();
             // one row tile every three steps, the last at steps 14 and 15
             constexpr int min_a = (t - 14 + 3 * (FM - 1)) / 3, min_at = 14 - 3 * (FM - 1);
@@ -261,9 +369,6 @@ __device__ __forceinline__ void experts_tile(const EgArgs& p, const Routing& r, 
                     if constexpr (kUnit) U[min_a][i] = dmin * M[i];
                     else T[min_a][i] = fmaf(dmin, M[i], T[min_a][i]);
                 }
-            }
-            if constexpr (!W::kAsync) {
-                if constexpr (t + 1 == 16) w.open();  // (the scales of the unit before are used up)
             }
             w.template step<(t + 1) % 16>(0, b[cur ^ 1]);
             if constexpr (!W::kQ8 && t != 0) {
@@ -562,7 +667,8 @@ bool experts_gemm_supported(const ExpertCall& c, const Routing& r) {
     const int64_t blocks = c.n * (c.k / epb);
     if (blocks * bpb > 0x7fffffff || eg_tiles(r, eg_rows(c, r), c.n, c.gated) > 0x7fffffff) return false;  // (offsets in a matrix, and the tiles' numbers, have 32 bits)
     const uintptr_t all = (uintptr_t)c.w[0] | (uintptr_t)c.expert_stride[0] | (c.gated ? (uintptr_t)c.w[1] | (uintptr_t)c.expert_stride[1] : 0);
-    if (c.encoding == QMM_Q4_0) return (all & 1) == 0;
+    // Q4_0: rows of whole units have to begin at multiples of four, others may begin two bytes later (an expert's, after an odd number of blocks)
+    if (c.encoding == QMM_Q4_0) return (all & 1) == 0 && (((uintptr_t)c.w[0] | (c.gated ? (uintptr_t)c.w[1] : 0)) & 3) == 0 && ((all & 3) == 0 || c.k % 256 != 0);
     if (all & 3) return false;
     return c.encoding != QMM_Q6_K || blocks % 2 == 0;  // (an odd last block would be read two bytes beyond its end)
 }

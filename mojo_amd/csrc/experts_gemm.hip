@@ -69,6 +69,7 @@ struct EgQ40 : NoOffsets {
         stage_lds = lds_address(at);
         w = t.w - ((uintptr_t)t.w & 2);
         row_bytes = t.k / 32 * Q4_0_BPB;
+        d[7] = 0;
         const int step = row_bytes < kUnit ? 0 : 16;  // (the only unit is partial: what is asked for in advance and never looked at stays within the row)
 #pragma unroll
         for (int j = 0; j < kWide; j++) {
@@ -121,7 +122,7 @@ struct EgQ40 : NoOffsets {
         cur = b + (lane_ & 31) * kUnit;
         tail = g ? b + kTail + 4 * (lane_ & 31) : cur + 136;
         read_block<0>();
-        last = d[7];  // (the block before the next unit's still has to be scaled)
+        last = d[7];  // (the last block is scaled in the next unit)
 #pragma unroll
         for (int i = 0; i < 8; i++) d[i] = g ? 0u : (uint32_t)*(const uint16_t*)(cur + skew + 18 * i);
     }
@@ -236,12 +237,14 @@ __device__ __forceinline__ void experts_tile(const EgArgs& p, const Routing& r, 
         if constexpr (kHasSums) load16_to_lds(sums_src + (int64_t)unit * 32, (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds0 + L::kS + (buf * FM + sums_tile) * 1024)));
     };
 
-    float16v T[FM], P[FM], M, U[kUnit ? FM : 1];
+    float16v T[FM], P[FM], M, U[kUnit ? FM : 1], B[2][FM], S[FM];  // Q4_0: products of two blocks, scales
+    half8 scales[FM];
 #pragma unroll
     for (int a = 0; a < FM; a++)
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-            T[a][i] = P[a][i] = 0.0f;
+            T[a][i] = P[a][i] = B[1][a][i] = 0.0f;
+            scales[a][i & 7] = 0;
             if constexpr (kUnit) U[a][i] = 0.0f;
         }
     const float16v zero16 = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -276,11 +279,7 @@ __device__ __forceinline__ void experts_tile(const EgArgs& p, const Routing& r, 
         issue_weights(next, (u + 1) & 1);
         issue_sums(next, (u + 1) & 1);
         float dmin = 0.0f, dnext = 0.0f;
-        half8 scales[FM];
-        if constexpr (W::kQ8) {
-#pragma unroll
-            for (int a = 0; a < FM; a++) scales[a] = *(const half8*)(smem + L::kS + ((u & 1) * FM + a) * 1024 + lane * 16);
-        } else {
+        if constexpr (!W::kQ8) {
             dnext = w.scale(0);
             if constexpr (W::kMin && !HILO) dmin = w.min_scale(0);
         }
@@ -310,19 +309,19 @@ __device__ __forceinline__ void experts_tile(const EgArgs& p, const Routing& r, 
             }
             __builtin_amdgcn_sched_barrier(0);
             if constexpr (W::kQ8) {
+// The products of a block are scaled while the next one's run.  Its scales as a matrix: the row's scale in slot b times the weight's in the same slot.
+                constexpr int done = (t / 2 + 7) % 8, at = t / 2 % 2;
 #pragma unroll
-                for (int a = 0; a < FM; a++)
-#pragma unroll
-                    for (int q = 0; q < kPer; q++) P[a] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af[cur][a][q], b[cur][0], t % 2 ? P[a] : zero16, 0, 0, 0);
+                for (int a = 0; a < FM; a++) {
+                    B[at][a] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af[cur][a][0], b[cur][0], t % 2 ? B[at][a] : zero16, 0, 0, 0);
+                    if constexpr (t % 2 == 0) S[a] = __builtin_amdgcn_mfma_f32_32x32x16_f16(scales[a], w.template scale_operand<done>(0), zero16, 0, 0, 0);
+                }
                 if constexpr (t % 2 == 1) {
-                    // the scales of a block as a matrix: the row's scale in slot t / 2 times the weight's in the same slot
-                    const half8 dw = w.template scale_operand<t / 2>(0);
 #pragma unroll
                     for (int a = 0; a < FM; a++) {
-                        const float16v S = __builtin_amdgcn_mfma_f32_32x32x16_f16(scales[a], dw, zero16, 0, 0, 0);
 #pragma unroll
-                        for (int i = 0; i < 16; i++) U[a][i] = t == 1 ? P[a][i] * S[i] : fmaf(P[a][i], S[i], U[a][i]);
-                        if constexpr (t == 15) {
+                        for (int i = 0; i < 16; i++) U[a][i] = done == 0 ? B[at ^ 1][a][i] * S[a][i] : fmaf(B[at ^ 1][a][i], S[a][i], U[a][i]);
+                        if constexpr (done == 7) {
 #pragma unroll
                             for (int i = 0; i < 16; i++) T[a][i] += U[a][i];
                             asm volatile("" : "+v"(T[a]));
@@ -330,6 +329,10 @@ __device__ __forceinline__ void experts_tile(const EgArgs& p, const Routing& r, 
                             asm volatile("" : "+v"(U[a]));
                         }
                     }
+                }
+                if constexpr (t == 0) {
+#pragma unroll
+                    for (int a = 0; a < FM; a++) scales[a] = *(const half8*)(smem + L::kS + ((u & 1) * FM + a) * 1024 + lane * 16);
                 }
             } else if constexpr (t == 0) {
 #pragma unroll
@@ -371,8 +374,9 @@ __device__ __forceinline__ void experts_tile(const EgArgs& p, const Routing& r, 
                 }
             }
             w.template step<(t + 1) % 16>(0, b[cur ^ 1]);
-            if constexpr (!W::kQ8 && t != 0) {
-                constexpr int kMfma = FM * kPer * W::kPlanes, kValu = (W::kPlanes == 2 ? 28 : 12) + (min_add ? 16 : 0);  // spread evenly
+            if constexpr (W::kQ8 || t != 0) {
+                constexpr int kMfma = FM * kPer * W::kPlanes * (W::kQ8 && t % 2 == 0 ? 2 : 1);
+                constexpr int kValu = (W::kPlanes == 2 ? 28 : 12) + (min_add ? 16 : 0) + (W::kQ8 && t % 2 ? 16 * FM : 0);  // spread evenly
                 unrolled<kMfma + (min_now ? (HILO ? 2 : 1) : 0)>([&](auto) __attribute__((always_inline)) {
                     __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
                     __builtin_amdgcn_sched_group_barrier(0x2, (kValu + kMfma - 1) / kMfma, 0);
@@ -381,7 +385,14 @@ __device__ __forceinline__ void experts_tile(const EgArgs& p, const Routing& r, 
             __builtin_amdgcn_sched_barrier(0);
         });
     }
-    if constexpr (!W::kQ8) {
+    if constexpr (W::kQ8) {
+#pragma unroll
+        for (int a = 0; a < FM; a++) {
+            S[a] = __builtin_amdgcn_mfma_f32_32x32x16_f16(scales[a], w.template scale_operand<7>(0), zero16, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 16; i++) T[a][i] += fmaf(B[1][a][i], S[a][i], U[a][i]);
+        }
+    } else {
 #pragma unroll
         for (int a = 0; a < FM; a++)
 #pragma unroll
@@ -651,11 +662,14 @@ hipError_t run_gemm(const EgArgs& p, const Routing& r, int fm, bool hilo, hipStr
 
 // Rows of a group, in 32s, by what an expert has on average.  Few rows: more groups fill the part better, and less is computed for rows that are not there; many: a weight is unpacked once for more of them.
 // us with 32 / 64 / 128 rows, bf16 rows, 8 of 64 experts, 1024 x 2048: Q4_K 32 rows an expert 37 / 44 / 42, 64 56 / 55 / 56, 128 88 / 81 / 85, 192 120 / 104 / 105; Q6_K (two products a weight) 24 60 / 62 / 56,
-// 48 85 / 65 / 74, 128 160 / 120 / 118, 192 211 / 151 / 145; 2 of 8, 14336 x 4096: Q4_K 32 106 / 103 / 103, 64 171 / 157 / 155, 256 498 / 390 / 344; Q4_0 (no 128) 64 68 / 74, 96 96 / 87; fp32 rows Q4_K 48 69 / 73, 96 111 / 104.
+// 48 85 / 65 / 74, 128 160 / 120 / 118, 192 211 / 151 / 145; 2 of 8, 14336 x 4096: Q4_K 32 106 / 103 / 103, 64 171 / 157 / 155, 256 498 / 390 / 344; fp32 rows Q4_K 48 69 / 73, 96 111 / 104.
+// Q4_0 (no 128): 8 of 64, 1024 x 2048 gate and up 32 rows 50 / 55, 48 90 / 74, 64 89 / 77, 128 175 / 141; 2 of 8, 14336 x 4096 32 93 / 97, 48 154 / 130.  But a workgroup is bound by its own chain of steps: where
+// tiles of 64 rows are less than one and a half a compute unit, those of 32 fill it better: 4 of 16, 1408 x 2080, drawn 64 rows (264 tiles of 64) 34 / 42, 96 (352) 42 / 43, 128 (440) 54 / 45.
 int eg_rows(const ExpertCall& c, const Routing& r) {
     const int64_t mean = r.pairs / r.experts;
     const bool f32 = c.lhs_dtype == QMM_F32;
-    const int one = c.encoding == QMM_Q4_0 ? 80 : !f32 && (c.encoding == QMM_Q5_K || c.encoding == QMM_Q6_K) ? 24 : 48;
+    if (c.encoding == QMM_Q4_0) return mean <= 40 || (r.pairs / 64 + r.experts / 2) * ((c.n + 127) / 128) * (c.gated ? 2 : 1) < 384 ? 1 : 2;
+    const int one = !f32 && (c.encoding == QMM_Q5_K || c.encoding == QMM_Q6_K) ? 24 : 48;
     return std::min(mean <= one ? 1 : mean <= 160 ? 2 : 4, eg_most(c.encoding, f32));
 }
 

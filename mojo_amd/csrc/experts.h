@@ -45,7 +45,7 @@ __device__ __forceinline__ ExpertRows find_rows_of(const Routing& r, int lane, F
     int left = group - (__shfl(sum, owner) - __shfl(mine, owner)), e = owner * per;
     for (; e <= r.experts; e++) {
         const int first = offset_at(r, e), count = max(offset_at(r, e + 1) - first, 0), groups = (count + ROWS - 1) / ROWS;
-        if (left < groups) return {e, first + left * ROWS, min(ROWS, count - left * ROWS)};
+        if (left < groups) return left < 0 ? ExpertRows{0, 0, 0} : ExpertRows{e, first + left * ROWS, min(ROWS, count - left * ROWS)};  // (below 0: offsets of no sorted pairs, more groups than an int holds)
         left -= groups;
     }
     return {0, 0, 0};

@@ -1296,6 +1296,7 @@ int qmm_route_experts(const void* logits, int logits_dtype, int64_t stride, int6
     const int64_t need = qmm::experts_group_workspace_bytes(tokens * top, experts, top);
     if (need > 0 && (!workspace || workspace_bytes < need))
         return fail(QMM_ERR_WORKSPACE, "qmm_route_experts: workspace of %lld bytes required, %lld given", (long long)need, (long long)workspace_bytes);
+    if (need > 0 && !aligned(workspace, 16)) return fail(QMM_ERR_INVALID, "qmm_route_experts: workspace must be 16-byte aligned");
     return hip_status(qmm::launch_route_experts(logits, logits_dtype, stride, tokens, experts, top, scoring == QMM_SIGMOID, bias, renormalize != 0, scale, ids, weights, offsets, order,
                                                 workspace, (hipStream_t)stream),
                       "qmm_route_experts");
@@ -1308,6 +1309,7 @@ int qmm_group_experts(const int32_t* ids, int64_t pairs, int experts, int32_t* o
     const int64_t need = qmm::experts_group_workspace_bytes(pairs, experts, 1);
     if (need > 0 && (!workspace || workspace_bytes < need))
         return fail(QMM_ERR_WORKSPACE, "qmm_group_experts: workspace of %lld bytes required, %lld given", (long long)need, (long long)workspace_bytes);
+    if (need > 0 && !aligned(workspace, 16)) return fail(QMM_ERR_INVALID, "qmm_group_experts: workspace must be 16-byte aligned");
     return hip_status(qmm::launch_group_experts(ids, pairs, experts, offsets, order, workspace, (hipStream_t)stream), "qmm_group_experts");
 }
 

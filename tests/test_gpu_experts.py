@@ -4,7 +4,8 @@ import pytest
 import torch
 
 import experts_reference as R
-from mojo_amd import (ExpertRouting, QuantizationEncoding as QE, group_experts, qmatmul_experts, qmatmul_experts_sum, qmatmul_experts_swiglu, route_experts)
+from gguf_writer import write_gguf
+from mojo_amd import (ExpertRouting, GGUFWeights, QuantizationEncoding as QE, group_experts, qmatmul_experts, qmatmul_experts_sum, qmatmul_experts_swiglu, route_experts)
 
 pytestmark = pytest.mark.gpu
 GGUF = (QE.Q4_0, QE.Q4_K, QE.Q5_K, QE.Q6_K)
@@ -217,6 +218,19 @@ def test_q4_0_rows_of_any_number_of_blocks(k, tokens):
     check(qmatmul_experts_swiglu(QE.Q4_0, c.lhs.to(DEV), c.gpu(0), c.gpu(1), c.routing), *silu_bound(*c.products(0), *c.products(1)), torch.float32)
 
 
+@pytest.mark.parametrize("k", (32, 96, 256, 288, 2080))
+@pytest.mark.parametrize("n, pad", ((71, 0), (71, 2), (72, 2), (33, 4)))
+@pytest.mark.parametrize("tokens", (1, 30, 140, 300))
+def test_q4_0_matrices_that_begin_between_multiples_of_four(k, n, pad, tokens):
+    """Blocks are 18 bytes: an expert's matrix, after an odd number of blocks or at a distance of its own, begins two bytes behind a multiple of four."""
+    c = Case(QE.Q4_0, tokens, 5, 2, n, k, torch.bfloat16)
+    size = n * k // 32 * 18
+    room = torch.full((5 * (size + pad),), 255, dtype=torch.uint8, device=DEV)
+    w = room[: 5 * (size + pad)].as_strided((5, n, k // 32 * 18), (size + pad, k // 32 * 18, 1))
+    w.copy_(c.gpu())
+    check(qmatmul_experts(QE.Q4_0, c.lhs.to(DEV), w, c.routing), *c.products(), torch.float32)
+
+
 @pytest.mark.parametrize("encoding", GGUF, ids=lambda e: e.name)
 @pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16))
 @pytest.mark.parametrize("tokens", (1, 4, 80))
@@ -335,6 +349,16 @@ def test_a_block_end_to_end():
     size = torch.stack([hb[c.ids == e].abs().sum(-1).max() * wd[e].abs().max() if (c.ids == e).any() else torch.tensor(0.0) for e in range(experts)]).max()
     want = c.lhs.double() + (weights[..., None] * y).sum(1)
     check(out, want, (weights[..., None] * yb).sum(1) + size + 2.0 ** 6 * R.U * (weights[..., None] * y).abs().sum(1) + 5 * R.U * want.abs(), torch.float32)
+
+
+def test_the_experts_of_a_gguf_file(tmp_path):
+    """The 3-D tensors as the reader hands them out."""
+    c = Case(QE.Q4_K, 20, 4, 2, 64, 512, torch.bfloat16, mats=2)
+    path = write_gguf(tmp_path / "experts.gguf", [], [(name, [512, 64, 4], 12, p.numpy().tobytes()) for name, p in zip(("gate", "up"), c.packed)])
+    file = GGUFWeights(path)
+    gate, up = (file.tensor(name, DEV) for name in ("gate", "up"))
+    assert gate.shape == c.packed[0].shape and file.encoding("gate") == QE.Q4_K
+    check(qmatmul_experts_swiglu(file.encoding("gate"), c.lhs.to(DEV), gate, up, c.routing), *silu_bound(*c.products(0), *c.products(1)), torch.float32)
 
 
 def test_refusals():

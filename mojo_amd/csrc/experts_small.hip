@@ -32,8 +32,9 @@ EsPlan es_plan(int encoding, int mrows, int64_t tiles, int64_t groups_y, int64_t
     p.waves = (int)((nblk + p.groups - 1) / p.groups);
     const int per_cu = std::max(1, kSmallWaves / p.waves);
     const int64_t places = std::max<int64_t>(1, (int64_t)compute_units() * per_cu / groups_y);
-    p.per = (int)std::min<int64_t>((tiles + places - 1) / places, 16);
-    p.grid = (int)((tiles + p.per - 1) / p.per);
+    const int64_t most = std::min<int64_t>((tiles + places - 1) / places, 16);
+    p.grid = (int)((tiles + most - 1) / most);
+    p.per = (int)((tiles + p.grid - 1) / p.grid);  // (small_body counts on `per` tiles or one less for every workgroup: (per - 1) grid < tiles)
     const int slot = encoding == QMM_Q4_0 || encoding == QMM_Q4_K ? SmallItem<QMM_Q4_K>::kSlot : encoding == QMM_Q5_K ? SmallItem<QMM_Q5_K>::kSlot : SmallItem<QMM_Q6_K>::kSlot;
     const int lr = mrows <= 4 ? 1 : mrows / 4, ring = p.waves * 2 * slot, bytes = (p.waves + (p.groups > 1 ? 1 : 0)) * lr * 256;
     p.chunk = std::min(std::min(p.per, 254), (kLdsPerCu / per_cu - ring) / bytes);

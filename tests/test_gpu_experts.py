@@ -218,6 +218,18 @@ def test_q4_0_rows_of_any_number_of_blocks(k, tokens):
     check(qmatmul_experts_swiglu(QE.Q4_0, c.lhs.to(DEV), c.gpu(0), c.gpu(1), c.routing), *silu_bound(*c.products(0), *c.products(1)), torch.float32)
 
 
+@pytest.mark.parametrize("n", (264, 280, 297, 376, 952))
+def test_many_experts_with_a_few_rows_of_more_tiles_than_a_workgroup_takes(n):
+    """128 experts (four different ones over and over) whose tiles do not go into the workgroups evenly."""
+    c = Case(QE.Q4_K, 70, 4, 1, n, 2304, torch.bfloat16, mats=2)
+    ids = R.choose(torch.randn(70, 128, generator=c.g), 4, "softmax", True)[0]
+    routing = group_experts(ids.to(DEV), torch.ones(ids.shape, device=DEV), 128)
+    gate, up = (c.gpu(i)[torch.arange(128, device=DEV) % 4] for i in (0, 1))
+    products = [R.products(QE.Q4_K, c.lhs, w, ids % 4) for w in c.w]
+    check(qmatmul_experts(QE.Q4_K, c.lhs.to(DEV), gate, routing), *products[0], torch.float32)
+    check(qmatmul_experts_swiglu(QE.Q4_K, c.lhs.to(DEV), gate, up, routing), *silu_bound(*products[0], *products[1]), torch.float32)
+
+
 @pytest.mark.parametrize("k", (32, 96, 256, 288, 2080))
 @pytest.mark.parametrize("n, pad", ((71, 0), (71, 2), (72, 2), (33, 4)))
 @pytest.mark.parametrize("tokens", (1, 30, 140, 300))

@@ -91,17 +91,22 @@ __device__ __forceinline__ void wave_join(LpState& a, int lane) {
 
 // One step of a bitonic sort over the lanes: the larger of a pair to the lane that wants it.
 template <int MASK>
+__device__ __forceinline__ void exchange(float& v, int lane, bool larger) {
+    const float o = lane_xor<MASK>(v, lane);
+    v = larger ? fmaxf(v, o) : fminf(v, o);
+}
+template <int MASK>
 __device__ __forceinline__ void exchange(uint64_t& v, int lane, bool larger) {
     const uint64_t o = (uint64_t)lane_xor<MASK>((uint32_t)(v >> 32), lane) << 32 | lane_xor<MASK>((uint32_t)v, lane);
     v = (v > o) == larger ? v : o;
 }
-template <int SIZE, int MASK>
-__device__ __forceinline__ void merge_step(uint64_t& v, int lane) {
+template <int SIZE, int MASK, typename V>
+__device__ __forceinline__ void merge_step(V& v, int lane) {
     exchange<MASK>(v, lane, ((lane & MASK) == 0) == (SIZE == 64 || (lane & SIZE) == 0));
     if constexpr (MASK > 1) merge_step<SIZE, MASK / 2>(v, lane);
 }
-template <int SIZE = 2>
-__device__ __forceinline__ void sort64(uint64_t& v, int lane) {  // falling
+template <int SIZE = 2, typename V>
+__device__ __forceinline__ void sort64(V& v, int lane) {  // falling
     merge_step<SIZE, SIZE / 2>(v, lane);
     if constexpr (SIZE < 64) sort64<SIZE * 2>(v, lane);
 }
@@ -143,6 +148,23 @@ __device__ __forceinline__ void top_keys(int count, int top, uint64_t* lists, in
         }
     }
     merge_waves<WAVES>(mine, lists, wave, lane);
+}
+
+// Nearly always there is a shorter way: of 64 numbers, each the largest of a share of the values, the top-th largest is a bound that at least `top` values reach, and hardly more (20 of them: 24 at random).
+// Those that do are gathered in any order and sorted once.  With more than kLpFew wanted the bound lets too many through; if more than 64 reach it (values that are equal, a mask), the long way is taken.
+constexpr int kLpFew = 32;
+// The gathered keys, falling, in lists[0 .. 63]; false: there were too many.
+__device__ __forceinline__ bool sort_gathered(uint64_t* lists, const int* taken, int wave, int lane) {
+    __syncthreads();
+    const int count = *taken;
+    if (count > 64) return false;
+    if (wave == 0) {
+        uint64_t v = lane < count ? lists[lane] : 0;
+        sort64(v, lane);
+        lists[lane] = v;
+    }
+    __syncthreads();
+    return true;
 }
 
 // The largest of three (no NaN among the results unless all are); the compiler's own would first make each value a quiet one.
@@ -232,6 +254,8 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(const T* __restric
     extern __shared__ __attribute__((aligned(16))) float runs[];
     __shared__ uint64_t lists[kLpThreads];
     __shared__ LpState waves[kLpWaves];
+    __shared__ int picked, taken;
+    if (threadIdx.x == 0) picked = taken = 0;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), part = (int)blockIdx.y;
     const int64_t row_number = blockIdx.x;
     const LpRow<T> row(logits + row_number * stride, vocab);
@@ -356,8 +380,49 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(const T* __restric
         const LpState b = waves[w];
         join(a, b);
     }
-    if (wanted) {
-        const int count = (end - first + 3) / 4;  // runs of this part
+    const int count = (end - first + 3) / 4;  // runs of this part
+    bool found = !wanted;
+    if (wanted && out.top <= kLpFew && count >= 64 && a.s == a.s) {
+        // run r belongs to share r mod 64
+        float* const shares = (float*)(lists + kLpThreads / 2);
+        float most = -__builtin_inff();
+        for (int run = threadIdx.x; run < count; run += kLpThreads) most = fmaxf(most, runs[run]);
+        shares[threadIdx.x] = most;
+        __syncthreads();
+        most = shares[lane];
+#pragma unroll
+        for (int w = 1; w < kLpWaves; w++) most = fmaxf(most, shares[w * 64 + lane]);
+        sort64(most, lane);
+        const float bound = __shfl(most, out.top - 1);
+        // the runs that reach it, then their values, a load a thread
+        if (bound > -__builtin_inff()) {
+            for (int run = threadIdx.x; run < count && *(volatile int*)&picked <= 64; run += kLpThreads) {
+                if (runs[run] < bound) continue;
+                const int at = atomicAdd(&picked, 1);
+                if (at < 64) ((int*)(lists + 64))[at] = run;
+            }
+        } else if (threadIdx.x == 0) {
+            picked = 65;  // (every value does)
+        }
+        __syncthreads();
+        const int v = picked <= 64 && (int)threadIdx.x < 4 * picked ? first + 4 * ((int*)(lists + 64))[threadIdx.x >> 2] + (int)(threadIdx.x & 3) : end;
+        if (v < end) {
+            float x[kPer];
+            LpRow<T>::unpack(row.whole(v) ? *(const lp_u4*)(row.aligned + (int64_t)v * kPer) : row.edge(v), x);  // (-inf where the row has no value)
+            int reached = 0;
+#pragma unroll
+            for (int i = 0; i < kPer; i++) reached += x[i] >= bound;
+            int at = reached ? atomicAdd(&taken, reached) : 0;
+#pragma unroll
+            for (int i = 0; i < kPer; i++) {
+                if (!(x[i] >= bound)) continue;
+                if (at < 64) lists[at] = key_of(x[i], (uint32_t)(v * kPer + i - row.skew));
+                at++;
+            }
+        }
+        found = picked <= 64 && sort_gathered(lists, &taken, wave, lane);
+    }
+    if (!found) {
         if (a.s != a.s) {
             // There is a NaN.  (One that signals would have hidden its neighbours from the maxima above.)
             for (int run = threadIdx.x; run < count; run += kLpThreads) {
@@ -406,6 +471,11 @@ template <typename T, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void logprobs_join_kernel(const T* __restrict__ logits, int64_t stride, int vocab, int parts, const LpState* __restrict__ states,
                                                                           const uint64_t* __restrict__ keys, LpOut out) {
     __shared__ uint64_t lists[64 * WAVES];
+    __shared__ int taken;
+    if (WAVES > 1) {
+        if (threadIdx.x == 0) taken = 0;
+        __syncthreads();
+    }
     const int lane = threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
     const int64_t row_number = blockIdx.x;
     const LpRow<T> row(logits + row_number * stride, vocab);
@@ -419,17 +489,46 @@ __global__ __launch_bounds__(64 * WAVES) void logprobs_join_kernel(const T* __re
     wave_join(a, lane);
     if (out.top > 0) {
         constexpr int kLists = 64 / WAVES > 8 ? 8 : 64 / WAVES;  // parts <= kLists WAVES
-        uint64_t v[kLists];
+        const uint64_t* const mine_of_row = keys + row_number * parts * out.top;
+        bool found = false;
+        if constexpr (WAVES > 1) {
+            if (out.top <= kLpFew && parts >= out.top) {
+                // the parts' largest
+                const int all = parts * out.top;
+                uint64_t v[kLpFew * 64 / (64 * WAVES)], most = lane < parts ? mine_of_row[lane * out.top] : 0;
 #pragma unroll
-        for (int i = 0; i < kLists; i++) {
-            const int part = wave + i * WAVES, at = i == 0 ? lane : 63 - lane;
-            v[i] = part < parts && at < out.top ? keys[(row_number * parts + part) * out.top + at] : 0;
+                for (int i = 0; i < (int)(sizeof(v) / 8); i++) {
+                    const int at = (int)threadIdx.x + i * 64 * WAVES;
+                    v[i] = at < all ? mine_of_row[at] : 0;
+                }
+                sort64(most, lane);
+                const uint64_t bound = shfl64(most, out.top - 1);
+                if (bound) {
+#pragma unroll
+                    for (int i = 0; i < (int)(sizeof(v) / 8); i++)
+                        if (v[i] >= bound) {
+                            const int at = atomicAdd(&taken, 1);
+                            if (at < 64) lists[at] = v[i];
+                        }
+                } else if (threadIdx.x == 0) {
+                    taken = 65;
+                }
+                found = sort_gathered(lists, &taken, wave, lane);
+            }
         }
-        uint64_t mine = v[0];
+        if (!found) {
+            uint64_t v[kLists];
 #pragma unroll
-        for (int i = 1; i < kLists; i++)
-            if (wave + i * WAVES < parts) merge64(mine, v[i], lane);
-        merge_waves<WAVES>(mine, lists, wave, lane);
+            for (int i = 0; i < kLists; i++) {
+                const int part = wave + i * WAVES, at = i == 0 ? lane : 63 - lane;
+                v[i] = part < parts && at < out.top ? mine_of_row[part * out.top + at] : 0;
+            }
+            uint64_t mine = v[0];
+#pragma unroll
+            for (int i = 1; i < kLists; i++)
+                if (wave + i * WAVES < parts) merge64(mine, v[i], lane);
+            merge_waves<WAVES>(mine, lists, wave, lane);
+        }
     }
     finish_row(row_number, row, a, token, lists, out);
 }

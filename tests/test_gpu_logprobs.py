@@ -21,7 +21,7 @@ def check(got, logits, tokens, top):
         assert g.shape == w.shape
         least = 128 * z.shape[-1] * 2.0 ** (-126 + z.amax(-1).abs().clamp(max=2.0 ** 30) * 2.0 ** -24)
         limit = 2.0 ** 6 * R.U * size + least.reshape(-1, *[1] * (size.dim() - 1))
-        error = (g - w).abs()
+        error = torch.where(g == w, 0.0, (g - w).abs())  # (-inf has to be -inf)
         assert (error <= limit).all(), f"{(error / limit).max():.3g} of the bound"
     if top:
         assert torch.equal(got.top_ids.cpu(), want[2])
@@ -62,6 +62,24 @@ def test_alternatives_do_not_depend_on_where_they_lie(vocab, order):
     tokens = torch.tensor([0, vocab - 1])
     for dtype in (torch.float32, torch.bfloat16):
         check(logprobs(x.to(dtype).to(DEV), tokens.to(DEV), 40), x.to(dtype), tokens, 40)
+
+
+@pytest.mark.parametrize("rows, vocab", ((2, 9000), (2, 150000), (1100, 9000)))
+@pytest.mark.parametrize("order", ("rising", "falling", "equal", "late", "steps", "mask", "few", "clusters"))
+@pytest.mark.parametrize("top", (1, 20, 32))
+def test_a_few_alternatives_do_not_depend_on_where_they_lie(rows, vocab, order, top):
+    """One workgroup a row and many; values of which more than there is room for are equal, masked, or next to each other."""
+    i = torch.arange(vocab, dtype=torch.float32)
+    x = {"rising": i / vocab, "falling": -i / vocab, "equal": torch.full((vocab,), 2.5), "late": torch.where(i >= vocab - 30, i / vocab, -3 - i / vocab), "steps": torch.floor(i / 7) % 5,
+         "mask": torch.where(i % 700 == 3, i / vocab, -torch.inf), "few": torch.where(i < 9, -i, -torch.inf), "clusters": torch.where(i % 2000 < 40, 1 + i / vocab, -i / vocab)}[order]
+    x = x.expand(3, -1).contiguous()
+    tokens = torch.tensor([0, vocab - 1, 3])
+    for dtype in (torch.float32, torch.bfloat16):
+        got = logprobs(x.to(dtype).to(DEV).repeat(rows // 2, 1)[:rows], tokens.to(DEV).repeat(rows // 2)[:rows], top)
+        last = (rows - 1) // 3 * 3 if rows > 3 else 0
+        n = min(3, rows - last)
+        check(type(got)(*(t[last:last + n] for t in got)), x[:n].to(dtype), tokens[:n], top)
+        assert rows == 2 or all(torch.equal(t[:999].reshape(333, 3, -1), t[:3].reshape(1, 3, -1).expand(333, -1, -1)) for t in got)
 
 
 def test_nearly_certain_rows_keep_their_digits():

@@ -14,7 +14,7 @@
 // The time does not depend on the values, where a list that every larger value is put into takes a row in rising order apart.
 //
 // What bounds it: with many rows the loads (a row is read once; the chosen runs again, from L2).  With few, the way through two launches: parts of a row go to several workgroups until
-// they are enough for the part, and one workgroup a row joins them.
+// they are enough for the part, and one workgroup a row joins them (lp_plan).
 #include <algorithm>
 
 #include "experts.h"
@@ -536,10 +536,12 @@ __global__ __launch_bounds__(64 * WAVES) void logprobs_join_kernel(const T* __re
 struct LpPlan {
     int per, parts;
 };
-// Workgroups a row: as few as make the runs of one fit its LDS (33 for QMM_MAX_VOCAB fp32 values), and until there are four for each compute unit, each with a load for every thread; 64 at most.
+// Workgroups a row: as few as make the runs of one fit its LDS (33 for QMM_MAX_VOCAB fp32 values).  Beyond, one where a row is less than four steps of a workgroup (a second launch is 4 us, a step one), and
+// else until there is one for each compute unit, each with a load for every thread; 64 at most.  us with 1 / 2 / 8 / 32 workgroups a row, fp32, 5 alternatives: 1 row of 32000 11.1 / 12.4 / 12.0 / 13.2, of 65536
+// 15.2 / 14.7 / 12.7 / 12.3, of 128256 21.8 / 18.8 / 14.3 / 12.3; 32 rows of 128256 23.5 / 20.8 / 16.4 / 21.2; 400 rows 48.1 / 55.8 / 72.1 / 160.
 LpPlan lp_plan(int dtype, int64_t rows, int64_t vocab, int top) {
     const int64_t per_load = dtype == QMM_F32 ? 4 : 8, loads = (vocab + 2 * per_load - 2) / per_load;  // (of the worst alignment)
-    const int64_t fewest = (loads + 4 * kLpRuns - 1) / (4 * kLpRuns), enough = (4 * (int64_t)compute_units() + rows / 2) / rows, most = std::min<int64_t>(64, std::max<int64_t>(1, loads / kLpThreads));
+    const int64_t fewest = (loads + 4 * kLpRuns - 1) / (4 * kLpRuns), enough = (compute_units() + rows / 2) / rows, most = loads < 4 * kLpStep ? 1 : std::min<int64_t>(64, loads / kLpThreads);
     int64_t parts = std::max(fewest, std::min(enough, most));
     const int64_t per = ((loads + parts - 1) / parts + 3) / 4 * 4;
     parts = (loads + per - 1) / per;

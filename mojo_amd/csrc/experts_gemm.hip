@@ -7,6 +7,10 @@
 // LDS is sized for two workgroups on a compute unit: an expert's K is short (8 units of 256 here and there), and what surrounds the products (finding the rows, the way to the first loads, the results) is
 // hidden by the other one.  One workgroup of eight wavefronts x 256 columns instead: 2000 tokens, 8 of 64 experts, 1024 x 2048, Q4_K gate and up 205 us; matrix cores busy a third of the time.
 //
+// What bounds it: that case 187 us now (718 TFLOP/s), matrix cores busy 0.45 of it, vector units 0.53, two wavefronts a SIMD hide little of one behind the other; 9 % of the matrix instructions are for rows that are not
+// there, and some compute units have nothing left for the last 15 %.  256 rows for each of the 64: 806 TFLOP/s, what the dense staged GEMM reaches on 16384 rows.  Q6_K down 500 fp32 rows, four products a weight: 99 us,
+// matrix cores 0.47.  Q4_0 1408 x 2080, 301 rows, 4 of 16: 31 us, nine units of K one after the other, vector units 0.52.
+//
 // The grid counts groups of rows as if every expert's last one were a group more: how many rows an expert has is known on the device only.  A workgroup looks for its group in the offsets
 // (a scan by one wavefront's lanes) and leaves if there is none; a group with few rows runs the body for as many.
 //

@@ -8,7 +8,8 @@
 // lower lanes of its own, found by comparing the bits of the expert's number over the lanes.  No atomics decide a place, so two calls give the same order.  Up to 1024 pairs one launch does both;
 // more take a second one for the places.
 //
-// What bounds it: latency (one token: the way in, `top` reductions of some forty instructions one after the other, the way out).
+// What bounds it: latency (one token: the way in, `top` reductions of some forty instructions one after the other, the way out).  In a trace, one fp32 token, 8 of 64 experts 3.8 us; 4099 bf16 tokens, 8 of
+// 128 8.8 us (vector units busy 0.63) and 7.5 for the places, 15.6 for both as called.
 #include <algorithm>
 
 #include "experts.h"

@@ -1,8 +1,10 @@
 // The experts' products for every shape: one wavefront takes one weight row (gated: one of gate and the same of up) of one expert for up to four of the expert's rows, a value at a time on the vector units.
 //
-// What the matrix-core kernels do not take goes here: weights at odd addresses, Q6_K rows with an odd number of blocks.  What bounds it is the unpacking, some twenty instructions a weight.
+// What the matrix-core kernels do not take goes here: weights at odd addresses, Q6_K rows with an odd number of blocks.  What bounds it is the unpacking, some twenty instructions a weight:
+// 8 of 64 experts, 1024 x 2048 at an odd address, 1 / 16 / 64 bf16 tokens Q4_K 37 / 305 / 539 us, Q6_K 29 / 212 / 409, Q4_0 18 / 110 / 213.
 // Q4_0: the lhs as Q8_0 codes and block scales (fp16, held as fp32), made by a launch in front; integer block dots.
-// Also here: the weighted sum over the experts of a token, which ends the products of every kernel that leaves the pairs' results apart.
+// Also here: the weighted sum over the experts of a token, which ends the products of every kernel that leaves the pairs' results apart: 500 tokens, 8 experts,
+// 2048 columns 7.6 us in a trace, 41 MB (5.4 TB/s, most of it from the caches).
 #include <algorithm>
 
 #include "experts.h"

@@ -1,7 +1,8 @@
 // The experts' products with a few rows for each expert: the kernel for a few lhs rows (small_body.h), a workgroup's rows being some of an expert's pairs and its weights that expert's.  One launch, no workspace.
 //
 // Groups of up to MROWS pairs are counted over the experts (blockIdx.y; as many as there can be, those beyond the last leave at once), the tiles of 16 weight rows of each over blockIdx.x.  With one token
-// every pair is a group and nothing is looked up.  What bounds it is the way to the first product and then the weights, as in the kernel that it is made of.
+// every pair is a group and nothing is looked up.  What bounds it is the way to the first product and then the weights, as in the kernel that it is made of:
+// one bf16 token, 8 of 64, 1024 x 2048 Q4_K gate and up 6.9 us (18.9 MB; 4 us to the first product); 16 fp32 tokens, 2 of 8, 14336 x 4096 Q5_K 75 us, 4.7 TB/s.
 //
 // The weighted sum of a token whose experts all have rows of their own is a product too: the experts' super-blocks one after the other as one long K, each times its expert's weight, so that one launch ends
 // with the token's results (a second launch, for the sum, is 2.5 us and the pairs' results written and read).

@@ -11,10 +11,12 @@
 // Alternatives.  A value that is among the `top` largest lies in one of the `top` runs of neighbouring values (four lanes' loads: 16 fp32 or 32 bf16 values) with the largest maxima, equal ones by
 // rising index.  So the pass leaves the maximum of every run in LDS (two DPP steps a load), and what follows looks for the largest of few: of 16 runs together,
 // of the runs of the chosen ones, of the values of the chosen runs.  A key is the value's bits in an order that integers compare right, above the index inverted: equal values by rising index, no two keys alike.
-// The time does not depend on the values, where a list that every larger value is put into takes a row in rising order apart.
+// The time of this long way does not depend on the values, where a list that every larger value is put into takes a row in rising order apart.  Up to 32 alternatives there is a shorter one for nearly all rows
+// (sort_gathered): one row of 128256 14.4 -> 12.5 us, 1021 bf16 rows 68 -> 65.
 //
 // What bounds it: with many rows the loads (a row is read once; the chosen runs again, from L2).  With few, the way through two launches: parts of a row go to several workgroups until
-// they are enough for the part, and one workgroup a row joins them (lp_plan).
+// they are enough for the part, and one workgroup a row joins them (lp_plan).  1021 rows of 128256 bf16, 5 alternatives:
+// 65 us, 4.0 TB/s, vector units busy 0.85 of the time; 200 rows fp32 22 us, 4.6 TB/s; one row, 20 alternatives: 12.6 us.
 #include <algorithm>
 
 #include "experts.h"

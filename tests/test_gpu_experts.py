@@ -1,4 +1,7 @@
 """The router, the pairs sorted by expert, and the experts' products against 64 bits."""
+import math
+import random
+
 import numpy as np
 import pytest
 import torch
@@ -361,6 +364,41 @@ def test_a_block_end_to_end():
     size = torch.stack([hb[c.ids == e].abs().sum(-1).max() * wd[e].abs().max() if (c.ids == e).any() else torch.tensor(0.0) for e in range(experts)]).max()
     want = c.lhs.double() + (weights[..., None] * y).sum(1)
     check(out, want, (weights[..., None] * yb).sum(1) + size + 2.0 ** 6 * R.U * (weights[..., None] * y).abs().sum(1) + 5 * R.U * want.abs(), torch.float32)
+
+
+def drawn_shapes(count):
+    """Sizes over the whole range of the kernels' rules: few and many experts, rows of an expert from less than one to hundreds, one tile of columns to hundreds, one block of K to sixteen."""
+    rng = random.Random(20)
+    for _ in range(count):
+        experts = rng.choice((1, 2, 3, 5, 8, 16, 33, 60, 64, 100, 128, 160))
+        top = min(experts, rng.choice((1, 1, 2, 4, 6, 8)))
+        tokens = max(1, min(int(experts * math.exp(rng.uniform(math.log(0.3), math.log(300))) / top), 8000 // top))
+        encoding = rng.choice(GGUF)
+        k = 32 * rng.randrange(1, 90) if encoding == QE.Q4_0 and rng.random() < 0.5 else 256 * rng.choice((1, 1, 2, 2, 3, 4, 5, 7, 8, 9, 10, 11, 14, 16))
+        n = int(math.exp(rng.uniform(rng.choice((0.0, 3.0, 4.5)), math.log(min(6000, 6.2e6 / (min(experts, 4) * k), 2.0e9 / (tokens * top * k) + 40)))))
+        yield encoding, tokens, experts, top, n, k, rng.choice((torch.float32, torch.bfloat16)), rng.choice(("each", "each", "gated", "sum")), rng.random() < 0.3
+
+
+@pytest.mark.parametrize("shape", drawn_shapes(150), ids=lambda s: "-".join(str(getattr(v, "name", v)).replace("torch.", "") for v in s))
+def test_drawn_shapes(shape):
+    """Weights: up to four different experts over and over."""
+    encoding, tokens, experts, top, n, k, dtype, op, per_pair = shape
+    c = Case(encoding, tokens, min(experts, 4), 1, n, k, dtype, per_pair=False, mats=2 if op == "gated" else 1)
+    lhs = torch.randn(tokens, top, k, generator=c.g).to(dtype) if per_pair else c.lhs
+    ids, weights = R.choose(torch.randn(tokens, experts, generator=c.g) + torch.randn(1, experts, generator=c.g), top, "softmax", True)
+    ids[torch.rand(ids.shape, generator=c.g) < 0.05] = -1
+    routing = group_experts(ids.to(DEV), weights.float().to(DEV), experts)
+    w = [c.gpu(i)[torch.arange(experts, device=DEV) % c.w[0].shape[0]] for i in range(len(c.w))]
+    products = [R.products(encoding, lhs, x, torch.where(ids < 0, ids, ids % x.shape[0])) for x in c.w]
+    x = lhs.to(DEV)
+    if op == "gated":
+        check(qmatmul_experts_swiglu(encoding, x, w[0], w[1], routing), *silu_bound(*products[0], *products[1]), torch.float32)
+    elif op == "each":
+        check(qmatmul_experts(encoding, x, w[0], routing), *products[0], torch.float32)
+    else:
+        share = torch.where(ids < 0, torch.zeros_like(weights), weights).float().double()[..., None]
+        terms, bounds = (share * t for t in products[0])
+        check(qmatmul_experts_sum(encoding, x, w[0], routing), terms.sum(1), bounds.sum(1) + (top + 1) * R.U * terms.abs().sum(1), torch.float32)
 
 
 def test_the_experts_of_a_gguf_file(tmp_path):

@@ -16,9 +16,9 @@ namespace qmm {
 
 namespace {
 
-template <int ENC, int MROWS, typename AT, int MODE, int EX>
+template <int ENC, int MROWS, typename AT, int MODE, int EX, bool PART>
 __global__ __launch_bounds__(64 * kSmallWaves) void experts_small_kernel(MmMats mats, const AT* __restrict__ a, int m, int k, SmallCut cut, SmallExperts ex) {
-    small_body<ENC, MROWS, AT, MODE, EX>(mats, a, m, k, cut, ex);
+    small_body<ENC, MROWS, AT, MODE, EX, PART>(mats, a, m, k, cut, ex);
 }
 
 struct EsPlan {
@@ -27,7 +27,7 @@ struct EsPlan {
 };
 // tiles: of one group of rows; groups_y: groups of rows that are expected; nblk: super-blocks that a workgroup walks.  One round of workgroups if there are as many groups as expected, but no more than 16 tiles
 // each: a group more than expected would otherwise be a round more (2 of 8 experts, 14336 x 4096 Q4_K, 16 fp32 rows 65 us, without the bound 46 or 90, with 8 tiles 71).
-EsPlan es_plan(int encoding, int mrows, int64_t tiles, int64_t groups_y, int64_t nblk) {
+EsPlan es_plan(int encoding, int mrows, int64_t tiles, int64_t groups_y, int64_t nblk, bool part) {
     EsPlan p;
     p.groups = (int)((nblk + kSmallWaves - 1) / kSmallWaves);
     p.waves = (int)((nblk + p.groups - 1) / p.groups);
@@ -36,18 +36,18 @@ EsPlan es_plan(int encoding, int mrows, int64_t tiles, int64_t groups_y, int64_t
     const int64_t most = std::min<int64_t>((tiles + places - 1) / places, 16);
     p.grid = (int)((tiles + most - 1) / most);
     p.per = (int)((tiles + p.grid - 1) / p.grid);  // (small_body counts on `per` tiles or one less for every workgroup: (per - 1) grid < tiles)
-    const int slot = encoding == QMM_Q4_0 || encoding == QMM_Q4_K ? SmallItem<QMM_Q4_K>::kSlot : encoding == QMM_Q5_K ? SmallItem<QMM_Q5_K>::kSlot : SmallItem<QMM_Q6_K>::kSlot;
+    const int slot = encoding == QMM_Q4_0 || encoding == QMM_Q4_K ? SmallItem<QMM_Q4_K>::kSlot + (part ? 64 : 0) : encoding == QMM_Q5_K ? SmallItem<QMM_Q5_K>::kSlot : SmallItem<QMM_Q6_K>::kSlot;
     const int lr = mrows <= 4 ? 1 : mrows / 4, ring = p.waves * 2 * slot, bytes = (p.waves + (p.groups > 1 ? 1 : 0)) * lr * 256;
     p.chunk = std::min(std::min(p.per, 254), (kLdsPerCu / per_cu - ring) / bytes);
     p.lds = (size_t)ring + (size_t)p.chunk * bytes;
     return p;
 }
 
-template <int ENC, int MROWS, typename AT, int MODE, int EX>
-hipError_t run_small(const ExpertCall& c, const SmallExperts& ex, int64_t groups_y, int64_t expected, void* out, bool out_bf16, hipStream_t s) {
+template <int ENC, int MROWS, typename AT, int MODE, int EX, bool PART>
+hipError_t run_part(const ExpertCall& c, const SmallExperts& ex, int64_t groups_y, int64_t expected, void* out, bool out_bf16, hipStream_t s) {
     const int tile = MODE == kSmallGated ? 8 : 16;
-    const EsPlan p = es_plan(ENC, MROWS, (c.n + tile - 1) / tile, expected, c.k / 256 * (EX == kSmallOverExperts ? ex.r.top : 1));
-    const hipError_t e = allow_full_lds<experts_small_kernel<ENC, MROWS, AT, MODE, EX>>();
+    const EsPlan p = es_plan(ENC, MROWS, (c.n + tile - 1) / tile, expected, (c.k + 255) / 256 * (EX == kSmallOverExperts ? ex.r.top : 1), PART);
+    const hipError_t e = allow_full_lds<experts_small_kernel<ENC, MROWS, AT, MODE, EX, PART>>();
     if (e != hipSuccess) return e;
     MmMats mats{};
     for (int j = 0; j < kLanesMaxMats; j++) {
@@ -57,8 +57,15 @@ hipError_t run_small(const ExpertCall& c, const SmallExperts& ex, int64_t groups
     }
     mats.count = 1;
     const SmallCut cut{p.per, p.grid, (uint32_t)p.waves | (uint32_t)p.chunk << 8 | (uint32_t)out_bf16 << 16 | (uint32_t)p.groups << 18};
-    experts_small_kernel<ENC, MROWS, AT, MODE, EX><<<dim3((unsigned)p.grid, (unsigned)groups_y), dim3((unsigned)(64 * p.waves)), p.lds, s>>>(mats, (const AT*)c.lhs, MROWS, (int)c.k, cut, ex);
+    experts_small_kernel<ENC, MROWS, AT, MODE, EX, PART><<<dim3((unsigned)p.grid, (unsigned)groups_y), dim3((unsigned)(64 * p.waves)), p.lds, s>>>(mats, (const AT*)c.lhs, MROWS, (int)c.k, cut, ex);
     return hipGetLastError();
+}
+template <int ENC, int MROWS, typename AT, int MODE, int EX>
+hipError_t run_small(const ExpertCall& c, const SmallExperts& ex, int64_t groups_y, int64_t expected, void* out, bool out_bf16, hipStream_t s) {
+    if constexpr (ENC == QMM_Q4_0) {
+        if (c.k % 256) return run_part<ENC, MROWS, AT, MODE, EX, true>(c, ex, groups_y, expected, out, out_bf16, s);
+    }
+    return run_part<ENC, MROWS, AT, MODE, EX, false>(c, ex, groups_y, expected, out, out_bf16, s);
 }
 template <int ENC, int MROWS, typename AT>
 hipError_t run_small(const ExpertCall& c, const SmallExperts& ex, int64_t groups_y, int64_t expected, void* out, bool out_bf16, hipStream_t s) {
@@ -106,11 +113,11 @@ hipError_t run_sum(const ExpertCall& c, const SmallExperts& ex, void* out, bool 
 
 bool es_takes(const ExpertCall& c) {
     if (kernel_disabled("experts_small")) return false;
-    if (c.k % 256 || c.k > (1 << 20)) return false;
+    if ((c.k % 256 && (c.encoding != QMM_Q4_0 || c.k < 256)) || c.k > (1 << 20)) return false;
     const uintptr_t all = (uintptr_t)c.w[0] | (uintptr_t)c.expert_stride[0] | (c.gated ? (uintptr_t)c.w[1] | (uintptr_t)c.expert_stride[1] : 0);
     if (c.encoding == QMM_Q4_K || c.encoding == QMM_Q5_K) return (all & 15) == 0;
     if (all & 3) return false;
-    return c.encoding == QMM_Q4_0 || c.n * (c.k / 256) % 2 == 0;  // (loads of four bytes at least: the last block of a matrix has to end at a multiple of four)
+    return c.n * (c.encoding == QMM_Q4_0 ? c.k / 32 : c.k / 256) % 2 == 0;  // (loads of four bytes at least: the last block of a matrix has to end at a multiple of four)
 }
 
 }  // namespace
@@ -134,7 +141,7 @@ hipError_t launch_experts_small(const ExpertCall& c, const Routing& r, void* out
     }
 }
 
-bool experts_sum_small_wanted(const ExpertCall& c, const Routing& r) { return es_takes(c) && r.pairs == r.top && c.k / 256 * r.top / kSmallWaves < 0x1fff; }
+bool experts_sum_small_wanted(const ExpertCall& c, const Routing& r) { return es_takes(c) && r.pairs == r.top && (c.k + 255) / 256 * r.top / kSmallWaves < 0x1fff; }
 
 hipError_t launch_experts_sum_small(const ExpertCall& c, const Routing& r, const void* residual, int residual_dtype, void* out, bool out_bf16, hipStream_t s) {
     const SmallExperts ex{r, {c.expert_stride[0], c.expert_stride[1]}, c.lhs_top, residual, residual_dtype == QMM_BF16};

@@ -44,7 +44,9 @@ struct SmallCut {
     int per, stride;  // tiles (pairs of them) of a workgroup at most, workgroups across the tiles
     uint32_t packed;  // wavefronts; << 8: items (tile of a matrix, or of both) of a workgroup whose partial results fit LDS together; << 16: bf16 results; << 17: a group of K per workgroup; << 18: groups of a workgroup; << 31: several tiles of lhs rows
 };
-template <int ENC, int MROWS, typename AT, int MODE, int EX = kSmallNoExperts>
+// PART (Q4_0, experts): K is no multiple of 256 (but no less).  The last super-block of a row begins 256 columns before its end; of the lhs, what the one before has too is taken as zeros there.  Rows and
+// super-blocks begin at even addresses, loads to LDS want multiples of four: a row's nine pieces from the last such address on, and four bytes more that a row which begins two bytes later needs.
+template <int ENC, int MROWS, typename AT, int MODE, int EX = kSmallNoExperts, bool PART = false>
 __device__ __forceinline__ void small_body(const MmMats& mats, const AT* __restrict__ a, int m, int k, const SmallCut& cut, const SmallExperts& ex = SmallExperts{}) {
     using I = SmallItem<ENC>;
     constexpr bool kQ8 = ENC == QMM_Q4_0;                   // the lhs as Q8_0 codes and block scales
@@ -53,6 +55,8 @@ __device__ __forceinline__ void small_body(const MmMats& mats, const AT* __restr
     constexpr int RN = LR * PL;
     constexpr int kPass = std::min(MROWS, 4 / PL);          // lhs rows that change lanes together
     static_assert(RN <= 4, "operand rows");
+    static_assert(!PART || (kQ8 && EX != kSmallNoExperts), "partial super-blocks");
+    constexpr int kSlot = I::kSlot + (PART ? 64 : 0), kLoads = I::kLoads + (PART ? 1 : 0);
     constexpr bool kMin = ENC == QMM_Q4_K || ENC == QMM_Q5_K;
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     const int tid = threadIdx.x, lane = tid & 63;
@@ -60,7 +64,7 @@ __device__ __forceinline__ void small_body(const MmMats& mats, const AT* __restr
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = (int)(cut.packed & 0xffu), chunk = (int)(cut.packed >> 8) & 0xff, per = cut.per, stride = cut.stride;
     const bool out_bf16 = (cut.packed >> 16) & 1, apart = (cut.packed >> 17) & 1;
     const int nn = lane & 15, kg = lane >> 4;
-    const int row_blocks = k >> 8, nblk = EX == kSmallOverExperts ? row_blocks * ex.r.top : row_blocks, groups = (int)(cut.packed >> 18) & 0x1fff;
+    const int row_blocks = PART ? (k + 255) >> 8 : k >> 8, nblk = EX == kSmallOverExperts ? row_blocks * ex.r.top : row_blocks, groups = (int)(cut.packed >> 18) & 0x1fff;
     int share = (int)blockIdx.x, part = (int)blockIdx.y, row0 = 0;  // this workgroup's tiles, group of K, first lhs row
     if (MROWS == small_rows<AT>() && (cut.packed >> 31)) {
         // several tiles of lhs rows: those that read the same weights side by side (blockIdx.y) on one XCD (ids congruent mod 8), every XCD the same number of them
@@ -106,20 +110,20 @@ __device__ __forceinline__ void small_body(const MmMats& mats, const AT* __restr
     }
     // super-block sb of a row of the lhs; kSmallOverExperts: of the row that the token's expert sb / row_blocks gets
     auto lhs_at = [&](int j, int sb) __attribute__((always_inline)) -> const AT* {
-        if constexpr (EX == kSmallByExpert) return a + (int64_t)lhs_rows[j] * k + sb * 256;
+        if constexpr (EX == kSmallByExpert) return a + (int64_t)lhs_rows[j] * k + (PART ? min(sb * 256, k - 256) : sb * 256);
         if constexpr (EX == kSmallOverExperts) {
             const int of = sb / row_blocks;
-            return a + (int64_t)(((int)blockIdx.y * ex.r.top + of) / ex.lhs_top) * k + (sb - of * row_blocks) * 256;
+            return a + (int64_t)(((int)blockIdx.y * ex.r.top + of) / ex.lhs_top) * k + (PART ? min((sb - of * row_blocks) * 256, k - 256) : (sb - of * row_blocks) * 256);
         }
         return a + (int64_t)min(row0 + j, m - 1) * k + sb * 256;
     };
     // One group per workgroup (then groups is 1, and the operands of the first conversion serve every item), or all of them.  (A flag or a comparison of the group's number instead, as `groups > 1` below, took Q6_K 1184 x 1024
     // with 33 rows from 4.95 to 5.11 us.)
     const int g_first = apart ? part : 0, g_end = apart ? g_first + 1 : groups;
-    const uint32_t row_bytes = (uint32_t)(row_blocks * I::kBpb);
-    uint8_t* const ring = smem + wave * (2 * I::kSlot);
+    const uint32_t row_bytes = PART ? (uint32_t)(k / 32 * Q4_0_BPB) : (uint32_t)(row_blocks * I::kBpb);
+    uint8_t* const ring = smem + wave * (2 * kSlot);
     const uint32_t ring_lds = lds_address(ring);
-    float* const accs = (float*)(smem + waves * (2 * I::kSlot));  // [chunk][waves][LR][64]
+    float* const accs = (float*)(smem + waves * (2 * kSlot));  // [chunk][waves][LR][64]
     float* const totals = accs + chunk * waves * LR * 64;  // [chunk][LR][64], with more than one group
     // Weight rows of a matrix in a tile.  Gated, eight of gate and the same eight of up: a workgroup has results whole with half as many of them.  14336 x 4096 4 bf16 rows: seven such tiles for each
     // of 256 compute units, where 896 pairs of whole tiles were four (eight tiles) for each of 224, 15.3 -> 13.9 us; Q6_K 13824 x 5120 28.8 -> 26.9, Q4_K 1000 x 4096 3 rows 6.9 -> 5.8.  The same sums.
@@ -142,14 +146,17 @@ __device__ __forceinline__ void small_body(const MmMats& mats, const AT* __restr
         return j;
     };
     // piece p = lane + 64 i of an item: row p / kRowPieces
-    uint32_t full[I::kLoads];  // byte offset of the piece (Q6_K: of its row) in a tile that lies inside the matrix
-    uint32_t at_row = 0;       // Q6_K: where it begins in the row, eight bits each
+    uint32_t full[I::kLoads];  // byte offset of the piece (Q6_K, PART: of its row) in a tile that lies inside the matrix
+    uint32_t at_row = 0;       // Q6_K, PART: where it begins in the row, eight bits each
 #pragma unroll
     for (int i = 0; i < I::kLoads; i++) {
         const int p = min(lane + 64 * i, I::kPieces - 1), pr = p / I::kRowPieces, pc = p - pr * I::kRowPieces;
-        full[i] = (uint32_t)(pr % kTile) * row_bytes + (ENC == QMM_Q6_K ? 0u : 16u * (uint32_t)pc);
+        full[i] = (uint32_t)(pr % kTile) * row_bytes + (ENC == QMM_Q6_K || PART ? 0u : 16u * (uint32_t)pc);
         if constexpr (ENC == QMM_Q6_K) at_row |= (pc < 13 ? 16u * (uint32_t)pc : 196u) << (8 * i);
+        if constexpr (PART) at_row |= 16u * (uint32_t)pc << (8 * i);
     }
+    // PART: where super-block sb of a row begins
+    auto window = [&](int sb) __attribute__((always_inline)) { return min((uint32_t)sb * (uint32_t)I::kBpb, row_bytes - (uint32_t)I::kBpb); };
     auto issue = [&](int sb, int item, int slot) {
         int n0, n;
         const int j = matrix_of(item, n0, n);
@@ -160,7 +167,7 @@ __device__ __forceinline__ void small_body(const MmMats& mats, const AT* __restr
             sb -= of * row_blocks;
             expert_at = max(__builtin_amdgcn_readlane(token_ids, of), 0) * ex.stride[0];
         }
-        const uint8_t* const base = mats.w[j] + expert_at + (int64_t)n0 * row_bytes + (ENC == QMM_Q6_K ? 0 : sb * I::kBpb);
+        const uint8_t* const base = mats.w[j] + expert_at + (int64_t)n0 * row_bytes + (ENC == QMM_Q6_K || PART ? 0 : sb * I::kBpb);
         const uint8_t* const base2 = MODE == kSmallGated ? mats.w[1] + (base - mats.w[0]) + (EX == kSmallByExpert ? er.expert * (ex.stride[1] - ex.stride[0]) : 0) : base;
         const int last = n - 1 - n0;  // rows past the matrix repeat its last row (their results are dropped)
 #pragma unroll
@@ -171,12 +178,19 @@ __device__ __forceinline__ void small_body(const MmMats& mats, const AT* __restr
                 off -= (uint32_t)(pr - min(pr, last)) * row_bytes;
             }
             if constexpr (ENC == QMM_Q6_K) off = ((off + (uint32_t)(sb * Q6_K_BPB)) & ~3u) + ((at_row >> (8 * i)) & 0xffu);
+            if constexpr (PART) off = ((off + window(sb)) & ~3u) + ((at_row >> (8 * i)) & 0xffu);
             if (i < I::kLoads - 1 || I::kPieces % 64 == 0 || lane < I::kPieces - 64 * (I::kLoads - 1)) {
-                const uint32_t to = ring_lds + slot * I::kSlot + i * 1024;
+                const uint32_t to = ring_lds + slot * kSlot + i * 1024;
                 constexpr int kGate = 8 * I::kRowPieces;  // pieces of the first of two matrices
                 if (MODE != kSmallGated || 64 * (i + 1) <= kGate) small_stream16(off, base, to);
                 else if (64 * i >= kGate) small_stream16(off, base2, to);
                 else load16_to_lds_once((lane + 64 * i < kGate ? base : base2) + off, to);
+            }
+        }
+        if constexpr (PART) {
+            if (lane < 16) {
+                const uint32_t at = (uint32_t)min(lane % kTile, last) * row_bytes + window(sb);
+                load4_to_lds((MODE != kSmallGated || lane < 8 ? base : base2) + (at & 2u ? (at & ~3u) + I::kBpb : at & ~3u), ring_lds + slot * kSlot + I::kSlot);
             }
         }
     };
@@ -275,6 +289,13 @@ __device__ __forceinline__ void small_body(const MmMats& mats, const AT* __restr
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the operands are in registers before the next item's load may overwrite the slot
     };
     const uint32_t a_lane = 4 * (uint32_t)sizeof(AT) * lane;
+    // PART: the columns of a row's last super-block that the one before has too
+    auto leave_out = [&](xraw_t (&xr)[MROWS], int sb) __attribute__((always_inline)) {
+        if (sb % row_blocks == row_blocks - 1 && 4 * lane < 256 * row_blocks - k) {
+#pragma unroll
+            for (int j = 0; j < MROWS; j++) xr[j] = xraw_t{};
+        }
+    };
 
     // first group: the lhs, then the first weights, which stay on their way while the lhs is converted.  (Straight-line code: nothing may move a register that such a load has
     // not filled yet.  A wavefront without a super-block, in the last group, takes the last one and drops it.)
@@ -285,10 +306,11 @@ __device__ __forceinline__ void small_body(const MmMats& mats, const AT* __restr
 #pragma unroll
         for (int j = 0; j < MROWS; j++) hidden_load(xr[j], a_lane, lhs_at(j, sb));
         issue(sb, 0, 0);
-        wait_vmcnt<I::kLoads>();
+        wait_vmcnt<kLoads>();
 #pragma unroll
         for (int j = 0; j < MROWS; j++) tie(xr[j]);
-        narrow(xr, ring + I::kSlot);
+        if constexpr (PART) leave_out(xr, sb);
+        narrow(xr, ring + kSlot);
     }
     // (constants of the unpack in vector registers: an and-or in one instruction takes no literal and one scalar at most)
     uint32_t m_low = ENC == QMM_Q5_K ? 0x01010101u : 0x03030303u, c54 = 0x54545454u;
@@ -311,7 +333,8 @@ __device__ __forceinline__ void small_body(const MmMats& mats, const AT* __restr
                 xraw_t xr[MROWS];
 #pragma unroll
                 for (int j = 0; j < MROWS; j++) xr[j] = *(const xraw_t*)((const uint8_t*)lhs_at(j, sb) + a_lane);
-                narrow(xr, ring + (slot ^ 1) * I::kSlot);
+                if constexpr (PART) leave_out(xr, sb);
+                narrow(xr, ring + (slot ^ 1) * kSlot);
             }
             for (int t = 0; t < ct; t++) {
                 // the next item: of the chunk, of the next group, of the next chunk
@@ -323,11 +346,11 @@ __device__ __forceinline__ void small_body(const MmMats& mats, const AT* __restr
                 if (nt < my_items) {
                     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (what was read from that slot is in registers)
                     issue(ng * waves + wave, nt, slot ^ 1);
-                    wait_vmcnt<I::kLoads>();
+                    wait_vmcnt<kLoads>();
                 } else {
                     wait_vmcnt<0>();
                 }
-                const uint8_t* const lb = ring + slot * I::kSlot + nn * I::kRow;
+                const uint8_t* const lb = ring + slot * kSlot + nn * I::kRow;
                 float v[LR];
                 if constexpr (kQ8) {
                     // codes less 8, times 16, as signed bytes: the dot products of a block come out exact; v = sum of dot / 16 * (d_w d_a), the product of two fp16 numbers exact in fp32
@@ -335,14 +358,20 @@ __device__ __forceinline__ void small_body(const MmMats& mats, const AT* __restr
                     float u[2][LR];  // two chains of sums
 #pragma unroll
                     for (int j = 0; j < LR; j++) u[0][j] = u[1][j] = 0.0f;
+                    // PART: the row begins 0 or 2 bytes into its pieces; behind the last of them, its four bytes more
+                    const uint32_t skew = PART ? ((uint32_t)(nn % kTile) * row_bytes + window(sb % row_blocks)) & 2u : 0u;
+                    const uint32_t behind = PART ? ((const uint32_t*)(ring + slot * kSlot + I::kSlot))[nn] : 0u;
 #pragma unroll
                     for (int b = 0; b < 8; b++) {
                         const int at = (18 * b + 2) >> 2;
                         uint32_t x;  // the block begins at 0 or 2 mod 4
-                        if ((18 * b + 2) % 4 == 0) x = l32[at + kg];
+                        if constexpr (PART) {
+                            const uint32_t* const p = l32 + (18 * b >> 2) + (b & 1) + kg + (b & 1 ? 0u : skew >> 1);
+                            x = __builtin_amdgcn_alignbyte(b == 7 && kg == 3 ? behind : p[1], p[0], b & 1 ? skew : skew ^ 2u);
+                        } else if ((18 * b + 2) % 4 == 0) x = l32[at + kg];
                         else x = __builtin_amdgcn_alignbyte(l32[at + kg + 1], l32[at + kg], 2);
                         const half2v dp = __builtin_bit_cast(half2v, l32[(18 * b) >> 2]);
-                        const _Float16 dw = (18 * b) % 4 ? dp.y : dp.x;
+                        const _Float16 dw = PART ? __builtin_bit_cast(_Float16, *(const uint16_t*)(lb + 18 * b + skew)) : (18 * b) % 4 ? dp.y : dp.x;
                         const u32x2 w = {((x << 4) & 0xF0F0F0F0u) ^ 0x80808080u, (x & 0xF0F0F0F0u) ^ 0x80808080u};
                         const ks_int4 dot = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, fc[b]), __builtin_bit_cast(long, w), ks_int4{0, 0, 0, 0}, 0, 0, 0);
 #pragma unroll

@@ -29,7 +29,10 @@ struct EsPlan {
 // each: a group more than expected would otherwise be a round more (2 of 8 experts, 14336 x 4096 Q4_K, 16 fp32 rows 65 us, without the bound 46 or 90, with 8 tiles 71).
 EsPlan es_plan(int encoding, int mrows, int64_t tiles, int64_t groups_y, int64_t nblk, bool part) {
     EsPlan p;
-    p.groups = (int)((nblk + kSmallWaves - 1) / kSmallWaves);
+    // Groups of four rows whose tiles are many: two workgroups of half as many wavefronts on a compute unit, one of which multiplies while the other ends.  (8 of 64, 1024 x 4096 Q4_K gate and up, one bf16 row an
+    // expert 49.7 -> 36.0 us, 2 of 8, 14336 x 4096 42.6 -> 37.4; Q6_K 77.5 -> 61.1.  With eight rows a group the lhs, narrowed for each of the groups of K, costs what that gains: Q6_K four rows an expert 86 -> 104.)
+    const int most_waves = mrows == 4 && tiles * groups_y > 8 * (int64_t)compute_units() ? kSmallWaves / 2 : kSmallWaves;
+    p.groups = (int)((nblk + most_waves - 1) / most_waves);
     p.waves = (int)((nblk + p.groups - 1) / p.groups);
     const int per_cu = std::max(1, kSmallWaves / p.waves);
     const int64_t places = std::max<int64_t>(1, (int64_t)compute_units() * per_cu / groups_y);
@@ -124,8 +127,9 @@ bool es_takes(const ExpertCall& c) {
 
 // Up to 8 rows an expert, or 12 where the GEMM unpacks more (bf16 rows but for Q4_K).  us, this kernel / the GEMM (with its preparation): 8 of 64 experts, 1024 x 2048, bf16 Q4_K 4 rows 19.8 / 28.0, 6 33.1 / 28.3,
 // 12 33.3 / 29.1; Q6_K 8 45.3 / 40.3, 12 45.5 / 57.2; Q5_K 8 35.5 / 36.9, 12 35.8 / 43.8; fp32 Q4_K 8 29.5 / 31.3, 12 44.6 / 32.1; 2 of 8, 14336 x 4096, bf16 Q4_K 8 74 / 79, 12 105 / 88; Q6_K 12 112 / 136, 16 155 / 137.
+// Q4_0: 8 of 64, 1024 x 2048 gate and up 8 bf16 rows 38.8 / 44.5; 1024 x 2080 (partial super-blocks) 6 47.1 / 48.0, 8 64.0 / 48.0.
 bool experts_small_wanted(const ExpertCall& c, const Routing& r) {
-    if (!es_takes(c) || es_mean(r) > (c.lhs_dtype == QMM_F32 || c.encoding == QMM_Q4_K ? 8.0 : 12.0)) return false;
+    if (!es_takes(c) || es_mean(r) > (c.k % 256 ? 6.5 : c.lhs_dtype == QMM_F32 || c.encoding == QMM_Q4_K ? 8.0 : 12.0)) return false;
     int64_t expected;
     const int rows = es_rows(c, r, expected);
     return es_groups(r, rows) <= 65535;

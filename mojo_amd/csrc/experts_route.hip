@@ -29,6 +29,7 @@ __device__ __forceinline__ uint64_t larger(uint64_t a, uint64_t b) { return a > 
 __device__ __forceinline__ uint64_t lane64(uint64_t v, int lane) {
     return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
 }
+__device__ __forceinline__ float lane32(float v, int lane) { return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), lane)); }
 __device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
     v = larger(v, dpp_move64<0xB1>(v));
     v = larger(v, dpp_move64<0x4E>(v));
@@ -62,13 +63,18 @@ __device__ __forceinline__ int route_token(const T* __restrict__ logits, const R
 #pragma unroll
     for (int i = 0; i < VPL; i++) {
         const int e = 64 * i + lane;
-        x[i] = e < c.experts ? load_f32(logits, token * c.stride + e) : -__builtin_inff();
+        x[i] = load_f32(logits, token * c.stride + min(e, c.experts - 1));  // (all loads at once)
     }
+#pragma unroll
+    for (int i = 0; i < VPL; i++) x[i] = 64 * i + lane < c.experts ? x[i] : -__builtin_inff();
     float m = x[0];
 #pragma unroll
     for (int i = 1; i < VPL; i++) m = fmaxf(m, x[i]);
-#pragma unroll
-    for (int mask = 32; mask; mask >>= 1) m = fmaxf(m, __shfl_xor(m, mask));
+    m = fmaxf(m, dpp_move<0xB1>(m));
+    m = fmaxf(m, dpp_move<0x4E>(m));
+    m = fmaxf(m, dpp_move<0x141>(m));
+    m = fmaxf(m, dpp_move<0x140>(m));
+    m = fmaxf(fmaxf(lane32(m, 0), lane32(m, 16)), fmaxf(lane32(m, 32), lane32(m, 48)));
     float chosen = 0.0f;  // lane j: the logit of the j-th choice
     int expert = -1;
     if (!c.bias) {

@@ -286,7 +286,7 @@ int qmm_matmul_rmsnorm(int encoding, const qmm_gptq_config* cfg, const void* x, 
  * rising index, -0 equal to 0, NaN below everything.  The score is softmax(logits) or sigmoid(logits); with `bias` (fp32[experts], may be null) the choice is made on
  * score + bias and the weight is that of the score alone.  renormalize: the weights are divided by their sum (a sum of 0: they are 0); all are multiplied by
  * `scale`.  A token whose logits are all -inf gets weights of 0.  experts up to 1024, top up to 64.
- * qmm_group_experts makes offsets and order from ids that come from elsewhere.
+ * qmm_group_experts makes offsets and order from ids that come from elsewhere.  Up to 2^28 pairs.
  * Both give the same order in every call (no atomics decide a place).  Workspace: qmm_experts_group_workspace_bytes (0 up to 1024 pairs; top: of a token, 1 for
  * qmm_group_experts).
  */
@@ -317,6 +317,7 @@ typedef struct qmm_routing {
  * inside a tensor that holds gate and up of an expert side by side).  lhs fp32 or bf16, lhs_rows = tokens (a token's row serves its `top` pairs) or
  * tokens top (a row for each pair).  out fp32, with QMM_FLAG_OUT_BF16 bf16.  Pairs without an expert get zeros (a sum leaves them out).  Only the experts that have rows are
  * read; nothing is asked of the device on the way, so the call can be captured.
+ * tokens top up to 2^23, n up to 2^18, k up to 2^20.
  * The routing's arrays may hold anything: what is not a pair or an expert is left out, nothing is read or written out of range.
  * Workspace: qmm_matmul_experts_workspace_bytes.
  */

@@ -102,17 +102,17 @@ __global__ __launch_bounds__(64 * kErWaves) void experts_rows_kernel(ErArgs a, R
 // The lhs of Q4_0: codes and block scales, 32 lanes a block.
 template <typename AT>
 __global__ __launch_bounds__(256) void experts_quantize_kernel(const AT* __restrict__ x, int64_t blocks, int8_t* __restrict__ codes, float* __restrict__ dscale) {
-    const int64_t block = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5;
-    if (block >= blocks) return;
     const int i = threadIdx.x & 31;
-    const float v = load_f32(x, block * 32 + i);
-    float amax = fabsf(v);
+    for (int64_t block = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); block < blocks; block += (int64_t)gridDim.x * 8) {
+        const float v = load_f32(x, block * 32 + i);
+        float amax = fabsf(v);
 #pragma unroll
-    for (int mask = 16; mask; mask >>= 1) amax = fmaxf(amax, __shfl_xor(amax, mask, 32));
-    uint16_t dh;
-    const float id = q8_0_block_rule<true>(amax, dh);
-    codes[block * 32 + i] = (int8_t)q8_0_code(v, id);
-    if (i == 0) dscale[block] = h2f(dh);
+        for (int mask = 16; mask; mask >>= 1) amax = fmaxf(amax, __shfl_xor(amax, mask, 32));
+        uint16_t dh;
+        const float id = q8_0_block_rule<true>(amax, dh);
+        codes[block * 32 + i] = (int8_t)q8_0_code(v, id);
+        if (i == 0) dscale[block] = h2f(dh);
+    }
 }
 
 // Four results a thread (n a multiple of four, aligned rows) or one.
@@ -160,8 +160,9 @@ hipError_t launch_experts_rows(const ExpertCall& c, const Routing& r, void* out,
         int8_t* const codes = (int8_t*)workspace;
         float* const dscale = (float*)(codes + (c.lhs_rows * c.k + 255) / 256 * 256);
         const int64_t blocks = c.lhs_rows * (c.k / 32);
-        if (c.lhs_dtype == QMM_F32) experts_quantize_kernel<<<dim3((unsigned)((blocks + 7) / 8)), dim3(256), 0, s>>>((const float*)c.lhs, blocks, codes, dscale);
-        else experts_quantize_kernel<<<dim3((unsigned)((blocks + 7) / 8)), dim3(256), 0, s>>>((const uint16_t*)c.lhs, blocks, codes, dscale);
+        const dim3 groups((unsigned)std::min<int64_t>((blocks + 7) / 8, 1 << 20));  // (a grid has up to 2^32 threads)
+        if (c.lhs_dtype == QMM_F32) experts_quantize_kernel<<<groups, dim3(256), 0, s>>>((const float*)c.lhs, blocks, codes, dscale);
+        else experts_quantize_kernel<<<groups, dim3(256), 0, s>>>((const uint16_t*)c.lhs, blocks, codes, dscale);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
         a.lhs = codes;

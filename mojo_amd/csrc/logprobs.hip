@@ -538,6 +538,7 @@ __global__ __launch_bounds__(64 * WAVES) void logprobs_join_kernel(const T* __re
 struct LpPlan {
     int per, parts;
 };
+constexpr int64_t kLpRows = 1 << 22;  // rows of a launch (a grid has up to 2^32 threads); more take one after the other, with the same plan
 // Workgroups a row: as few as make the runs of one fit its LDS (33 for QMM_MAX_VOCAB fp32 values).  Beyond, one where a row is less than four steps of a workgroup (a second launch is 4 us, a step one), and
 // else until there is one for each compute unit, each with a load for every thread; 64 at most.  us with 1 / 2 / 8 / 32 workgroups a row, fp32, 5 alternatives: 1 row of 32000 11.1 / 12.4 / 12.0 / 13.2, of 65536
 // 15.2 / 14.7 / 12.7 / 12.3, of 128256 21.8 / 18.8 / 14.3 / 12.3; 32 rows of 128256 23.5 / 20.8 / 16.4 / 21.2; 400 rows 48.1 / 55.8 / 72.1 / 160.
@@ -551,8 +552,7 @@ LpPlan lp_plan(int dtype, int64_t rows, int64_t vocab, int top) {
 }
 
 template <typename T>
-hipError_t run_logprobs(const T* logits, int dtype, int64_t stride, int64_t rows, int64_t vocab, const LpOut& out, void* workspace, hipStream_t s) {
-    const LpPlan p = lp_plan(dtype, rows, vocab, out.top);
+hipError_t run_logprobs(const T* logits, const LpPlan& p, int64_t stride, int64_t rows, int64_t vocab, const LpOut& out, void* workspace, hipStream_t s) {
     uint64_t* const keys = (uint64_t*)workspace;
     LpState* const states = (LpState*)(keys + rows * p.parts * out.top);
     const size_t lds = out.top > 0 ? (size_t)((p.per + 3) / 4) * 4 : 0;
@@ -567,15 +567,23 @@ hipError_t run_logprobs(const T* logits, int dtype, int64_t stride, int64_t rows
 }  // namespace
 
 int64_t logprobs_workspace_bytes(int dtype, int64_t rows, int64_t vocab, int top) {
+    rows = std::min(rows, kLpRows);
     const LpPlan p = lp_plan(dtype, rows, vocab, top);
     return p.parts == 1 ? 0 : rows * p.parts * ((int64_t)sizeof(LpState) + 8 * (int64_t)top);
 }
 
 hipError_t launch_logprobs(const void* logits, int dtype, int64_t stride, int64_t rows, int64_t vocab, const void* tokens, bool wide, int per_row, int top, float* chosen,
                            float* entropy, int32_t* top_ids, float* top_values, void* workspace, hipStream_t s) {
-    const LpOut out{tokens, wide, per_row, chosen, entropy, top_values, top_ids, top};
-    return dtype == QMM_F32 ? run_logprobs((const float*)logits, dtype, stride, rows, vocab, out, workspace, s)
-                            : run_logprobs((const uint16_t*)logits, dtype, stride, rows, vocab, out, workspace, s);
+    const LpPlan p = lp_plan(dtype, std::min(rows, kLpRows), vocab, top);
+    for (int64_t r0 = 0; r0 < rows; r0 += kLpRows) {
+        const int64_t n = std::min(rows - r0, kLpRows);
+        const LpOut out{tokens ? (const char*)tokens + r0 * per_row * (wide ? 8 : 4) : nullptr, wide, per_row, chosen ? chosen + r0 * per_row : nullptr, entropy + r0, top ? top_values + r0 * top : nullptr,
+                        top ? top_ids + r0 * top : nullptr, top};
+        const hipError_t e = dtype == QMM_F32 ? run_logprobs((const float*)logits + r0 * stride, p, stride, n, vocab, out, workspace, s)
+                                              : run_logprobs((const uint16_t*)logits + r0 * stride, p, stride, n, vocab, out, workspace, s);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace qmm

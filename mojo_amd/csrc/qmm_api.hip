@@ -43,7 +43,7 @@ int hip_status(hipError_t e, const char* what) {
 }
 
 // of the experts' products: pairs of a token and an expert; rows and columns of an expert's matrix
-constexpr int64_t kMostPairs = 1 << 28, kMostExpertRows = 1 << 18, kMostExpertColumns = 1 << 20;
+constexpr int64_t kMostPairs = 1 << 28, kMostProducts = 1 << 23, kMostExpertRows = 1 << 18, kMostExpertColumns = 1 << 20;
 
 bool aligned(const void* p, uintptr_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
 
@@ -1334,7 +1334,7 @@ int qmm_matmul_experts(int op, int encoding, const qmm_routing* routing, const v
     if (encoding == QMM_Q8_0 || encoding == QMM_Q8_K || encoding == QMM_GPTQ || !block_params(encoding, epb, bpb))
         return fail(QMM_ERR_INVALID, "qmm_matmul_experts: encoding %d is not a GGUF weight encoding", encoding);
     const int64_t tokens = routing->tokens, top = routing->top, experts = routing->experts;
-    if (experts < 1 || experts > QMM_MAX_EXPERTS || top < 1 || top > QMM_MAX_TOP || tokens < 1 || tokens > kMostPairs / top)
+    if (experts < 1 || experts > QMM_MAX_EXPERTS || top < 1 || top > QMM_MAX_TOP || tokens < 1 || tokens > kMostProducts / top)
         return fail(QMM_ERR_INVALID, "qmm_matmul_experts: %lld tokens, %lld of %lld experts", (long long)tokens, (long long)top, (long long)experts);
     if (n < 1 || n > kMostExpertRows || k < 1 || k > kMostExpertColumns || k % epb)
         return fail(QMM_ERR_INVALID, "qmm_matmul_experts: N=%lld (1 .. %lld) K=%lld (a multiple of %lld up to %lld)", (long long)n, (long long)kMostExpertRows, (long long)k, (long long)epb,

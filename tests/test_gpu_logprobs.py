@@ -82,6 +82,13 @@ def test_a_few_alternatives_do_not_depend_on_where_they_lie(rows, vocab, order, 
         assert rows == 2 or all(torch.equal(t[:999].reshape(333, 3, -1), t[:3].reshape(1, 3, -1).expand(333, -1, -1)) for t in got)
 
 
+def test_more_rows_than_a_launch_takes():
+    rows = 2 ** 22 + 5
+    x = torch.randn(rows, 3, generator=torch.Generator().manual_seed(9))
+    tokens = torch.arange(rows) % 3
+    check(logprobs(x.to(DEV), tokens.to(DEV), 1), x, tokens, 1)
+
+
 def test_nearly_certain_rows_keep_their_digits():
     x = torch.full((4, 70000), -30.0)
     for r, top in enumerate((0.0, 10.0, 60.0, 300.0)):

@@ -287,8 +287,8 @@ int qmm_matmul_rmsnorm(int encoding, const qmm_gptq_config* cfg, const void* x, 
  * score + bias and the weight is that of the score alone.  renormalize: the weights are divided by their sum (a sum of 0: they are 0); all are multiplied by
  * `scale`.  A token whose logits are all -inf gets weights of 0.  experts up to 1024, top up to 64.
  * qmm_group_experts makes offsets and order from ids that come from elsewhere.  Up to 2^28 pairs.
- * Both give the same order in every call (no atomics decide a place).  Workspace: qmm_experts_group_workspace_bytes (0 up to 1024 pairs; top: of a token, 1 for
- * qmm_group_experts).
+ * Both give the same order in every call (no atomics decide a place).  Workspace: qmm_experts_group_workspace_bytes (top: of a token, 1 for
+ * qmm_group_experts); none for a few tokens (64 pairs and fewer of up to 32 tokens), or up to 1024 pairs for qmm_group_experts.
  */
 enum qmm_scoring { QMM_SOFTMAX = 0, QMM_SIGMOID = 1 };
 #define QMM_MAX_EXPERTS 1024

@@ -64,7 +64,8 @@ __device__ __forceinline__ int pair_at(const Routing& r, int place) {
 }
 
 // experts_route.hip
-int64_t experts_group_workspace_bytes(int64_t pairs, int experts, int top);  // top: of a token (pairs that are grouped by themselves: 1)
+int64_t route_workspace_bytes(int64_t tokens, int experts, int top);
+int64_t group_workspace_bytes(int64_t pairs, int experts);
 hipError_t launch_route_experts(const void* logits, int dtype, int64_t stride, int64_t tokens, int experts, int top, bool sigmoid, const float* bias, bool renormalize, float scale,
                                 int32_t* ids, float* weights, int32_t* offsets, int32_t* order, void* workspace, hipStream_t s);
 hipError_t launch_group_experts(const int32_t* ids, int64_t pairs, int experts, int32_t* offsets, int32_t* order, void* workspace, hipStream_t s);

@@ -5,8 +5,8 @@
 // scores the choice is made in 64 bits, where no two scores that differ round to one.
 //
 // The sort is stable and counts: every workgroup counts its pairs by expert; what lies before a pair is the pairs of lower experts, those of its expert in workgroups and wavefronts before, and those in
-// lower lanes of its own, found by comparing the bits of the expert's number over the lanes.  No atomics decide a place, so two calls give the same order.  Up to 1024 pairs one launch does both;
-// more take a second one for the places.
+// lower lanes of its own, found by comparing the bits of the expert's number over the lanes.  No atomics decide a place, so two calls give the same order.  A few tokens, or 1024 pairs whose experts
+// are given, one launch does both; more take a second one for the places.
 //
 // What bounds it: latency (one token: the way in, `top` reductions of some forty instructions one after the other, the way out).  In a trace, one fp32 token, 8 of 64 experts 3.8 us; 4099 bf16 tokens, 8 of
 // 128 8.8 us (vector units busy 0.63) and 7.5 for the places, 15.6 for both as called.
@@ -256,7 +256,7 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(const T* __restric
     count_or_place(ids, t0 * c.top, t1 * c.top, c.experts, route_lds, offsets, order, blocks, wave, lane);
 }
 
-// Up to 64 pairs in all: one a lane.  Its place is the number of pairs before it; every thread counts the pairs of experts below some.
+// Up to 32 pairs in all, one a lane (64 took 9.1 us where the sort below takes 6).  Its place is the number of pairs before it; every thread counts the pairs of experts below some.
 template <int VPL, typename T>
 __global__ __launch_bounds__(kRouteThreads) void route_few_kernel(const T* __restrict__ logits, RouteCall c, int32_t* __restrict__ ids, float* __restrict__ weights, int32_t* __restrict__ offsets,
                                                                   int32_t* __restrict__ order) {
@@ -342,17 +342,17 @@ __global__ __launch_bounds__(kRouteThreads) void place_kernel(const int32_t* __r
     place_pairs(ids, first, from, to, experts, route_lds, start, order, wave, lane);
 }
 
-// Tokens (pairs, with top 1) of a workgroup: all, up to 1024 pairs; else one a wavefront and as many more as leave kRouteBlocks workgroups.
-int64_t route_per(int64_t tokens, int top) {
-    if (tokens * top <= kRouteThreads) return tokens;
-    const int64_t least = top == 1 ? kRouteThreads : kRouteWaves;
-    return std::max(least, (tokens + kRouteBlocks - 1) / kRouteBlocks);
-}
+// Tokens of a workgroup: all, up to two for each wavefront and 192 pairs; else one a wavefront and as many more as leave kRouteBlocks workgroups.  (A token after the other is 1 .. 2 us, a second launch 4: fp32
+// tokens, 3 of 64 experts 32 6.9 us in one workgroup, 33 8.9 in two launches, 304 36.4 in one, 9.3 in two; 8 of 64 24 8.3 in one, 32 10.5, 33 9.6 in two.)
+int64_t route_per(int64_t tokens, int top) { return tokens <= 2 * kRouteWaves && tokens * top <= 192 ? tokens : std::max<int64_t>(kRouteWaves, (tokens + kRouteBlocks - 1) / kRouteBlocks); }
+// Pairs of a workgroup, where the experts are given.
+int64_t group_per(int64_t pairs) { return pairs <= kRouteThreads ? pairs : std::max<int64_t>(kRouteThreads, (pairs + kRouteBlocks - 1) / kRouteBlocks); }
+int64_t counts_bytes(int64_t blocks, int experts) { return blocks > 1 ? blocks * counts_stride(experts) * 4 : 0; }
 size_t sort_lds(int experts) { return (size_t)(kRouteWaves + 2) * (experts + 1) * 4; }
 
 template <int VPL, typename T>
 hipError_t run_route(const T* logits, const RouteCall& c, int64_t per, int32_t* ids, float* weights, int32_t* offsets, int32_t* order, int32_t* blocks, hipStream_t s) {
-    if ((int64_t)c.tokens * c.top <= 64) {
+    if ((int64_t)c.tokens * c.top <= 32) {
         route_few_kernel<VPL, T><<<dim3(1), dim3((unsigned)(64 * std::min(c.tokens, kRouteWaves))), 0, s>>>(logits, c, ids, weights, offsets, order);
         return hipGetLastError();
     }
@@ -379,10 +379,8 @@ hipError_t run_places(const int32_t* ids, int64_t pairs, int experts, int64_t pe
 
 }  // namespace
 
-int64_t experts_group_workspace_bytes(int64_t pairs, int experts, int top) {
-    const int64_t tokens = pairs / top, per = route_per(tokens, top), blocks = per > 0 ? (tokens + per - 1) / per : 0;
-    return blocks > 1 ? blocks * counts_stride(experts) * 4 : 0;
-}
+int64_t route_workspace_bytes(int64_t tokens, int experts, int top) { return counts_bytes((tokens + route_per(tokens, top) - 1) / route_per(tokens, top), experts); }
+int64_t group_workspace_bytes(int64_t pairs, int experts) { return counts_bytes((pairs + group_per(pairs) - 1) / group_per(pairs), experts); }
 
 hipError_t launch_route_experts(const void* logits, int dtype, int64_t stride, int64_t tokens, int experts, int top, bool sigmoid, const float* bias, bool renormalize, float scale,
                                 int32_t* ids, float* weights, int32_t* offsets, int32_t* order, void* workspace, hipStream_t s) {
@@ -395,7 +393,7 @@ hipError_t launch_route_experts(const void* logits, int dtype, int64_t stride, i
 }
 
 hipError_t launch_group_experts(const int32_t* ids, int64_t pairs, int experts, int32_t* offsets, int32_t* order, void* workspace, hipStream_t s) {
-    const int64_t per = route_per(pairs, 1);
+    const int64_t per = group_per(pairs);
     int32_t* const blocks = per < pairs ? (int32_t*)workspace : nullptr;
     hipError_t e = allow_full_lds<group_kernel>();
     if (e != hipSuccess) return e;

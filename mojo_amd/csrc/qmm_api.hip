@@ -1282,7 +1282,7 @@ int64_t qmm_preferred_workspace_bytes(int op, int encoding, const qmm_gptq_confi
 
 int64_t qmm_experts_group_workspace_bytes(int64_t pairs, int experts, int top) {
     if (pairs <= 0 || experts <= 0 || top <= 0) return 0;
-    return qmm::experts_group_workspace_bytes(pairs, experts, top);
+    return std::max(qmm::route_workspace_bytes((pairs + top - 1) / top, experts, top), top == 1 ? qmm::group_workspace_bytes(pairs, experts) : 0);
 }
 
 int qmm_route_experts(const void* logits, int logits_dtype, int64_t stride, int64_t tokens, int experts, int top, int scoring, const float* bias, int renormalize, float scale,
@@ -1291,9 +1291,9 @@ int qmm_route_experts(const void* logits, int logits_dtype, int64_t stride, int6
     if (logits_dtype != QMM_F32 && logits_dtype != QMM_BF16) return fail(QMM_ERR_INVALID, "qmm_route_experts: logits must be f32 or bf16");
     if (experts < 1 || experts > QMM_MAX_EXPERTS || top < 1 || top > QMM_MAX_TOP || top > experts)
         return fail(QMM_ERR_INVALID, "qmm_route_experts: %d of %d experts (1 .. %d experts, 1 .. %d of them)", top, experts, QMM_MAX_EXPERTS, QMM_MAX_TOP);
-    if (tokens < 1 || tokens * top > kMostPairs || stride < experts) return fail(QMM_ERR_INVALID, "qmm_route_experts: %lld tokens, stride %lld", (long long)tokens, (long long)stride);
+    if (tokens < 1 || tokens > kMostPairs / top || stride < experts) return fail(QMM_ERR_INVALID, "qmm_route_experts: %lld tokens, stride %lld", (long long)tokens, (long long)stride);
     if (scoring != QMM_SOFTMAX && scoring != QMM_SIGMOID) return fail(QMM_ERR_INVALID, "qmm_route_experts: unknown scoring %d", scoring);
-    const int64_t need = qmm::experts_group_workspace_bytes(tokens * top, experts, top);
+    const int64_t need = qmm::route_workspace_bytes(tokens, experts, top);
     if (need > 0 && (!workspace || workspace_bytes < need))
         return fail(QMM_ERR_WORKSPACE, "qmm_route_experts: workspace of %lld bytes required, %lld given", (long long)need, (long long)workspace_bytes);
     if (need > 0 && !aligned(workspace, 16)) return fail(QMM_ERR_INVALID, "qmm_route_experts: workspace must be 16-byte aligned");
@@ -1306,7 +1306,7 @@ int qmm_group_experts(const int32_t* ids, int64_t pairs, int experts, int32_t* o
     if (!ids || !offsets || !order) return fail(QMM_ERR_INVALID, "qmm_group_experts: null pointer");
     if (experts < 1 || experts > QMM_MAX_EXPERTS || pairs < 1 || pairs > kMostPairs)
         return fail(QMM_ERR_INVALID, "qmm_group_experts: %lld pairs, %d experts (1 .. %d)", (long long)pairs, experts, QMM_MAX_EXPERTS);
-    const int64_t need = qmm::experts_group_workspace_bytes(pairs, experts, 1);
+    const int64_t need = qmm::group_workspace_bytes(pairs, experts);
     if (need > 0 && (!workspace || workspace_bytes < need))
         return fail(QMM_ERR_WORKSPACE, "qmm_group_experts: workspace of %lld bytes required, %lld given", (long long)need, (long long)workspace_bytes);
     if (need > 0 && !aligned(workspace, 16)) return fail(QMM_ERR_INVALID, "qmm_group_experts: workspace must be 16-byte aligned");

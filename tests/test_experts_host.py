@@ -30,7 +30,7 @@ def test_route_and_group_refusals(lib):
     for kw in ({"logits": None}, {"dtype": 2}, {"stride": 63}, {"tokens": 0}, {"experts": 1025, "stride": 2000}, {"experts": 0}, {"top": 0}, {"top": 65, "experts": 128, "stride": 128}, {"experts": 4},
                {"scoring": 2}, {"tokens": 1 << 60}):
         assert route(**kw) == -1 and "qmm_route_experts" in message(lib), kw
-    assert lib.qmm_experts_group_workspace_bytes(1024, 64, 8) == 0
+    assert lib.qmm_experts_group_workspace_bytes(64, 64, 8) == 0
     need = lib.qmm_experts_group_workspace_bytes(8 * 1000, 64, 8)
     assert need > 0 and route(tokens=1000, ws=P, ws_bytes=need - 1) == -4
     assert lib.qmm_group_experts(P, 0, 8, P, P, None, 0, None) == -1

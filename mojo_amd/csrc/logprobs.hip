@@ -107,10 +107,10 @@ __device__ __forceinline__ void merge_step(V& v, int lane) {
     exchange<MASK>(v, lane, ((lane & MASK) == 0) == (SIZE == 64 || (lane & SIZE) == 0));
     if constexpr (MASK > 1) merge_step<SIZE, MASK / 2>(v, lane);
 }
-template <int SIZE = 2, typename V>
-__device__ __forceinline__ void sort64(V& v, int lane) {  // falling
+template <int SIZE = 2, int COUNT = 64, typename V>
+__device__ __forceinline__ void sort64(V& v, int lane) {  // falling; the first COUNT lanes
     merge_step<SIZE, SIZE / 2>(v, lane);
-    if constexpr (SIZE < 64) sort64<SIZE * 2>(v, lane);
+    if constexpr (SIZE < COUNT) sort64<SIZE * 2, COUNT>(v, lane);
 }
 // a: falling; reversed: another falling list, last entry first.  The 64 largest of both, falling.
 __device__ __forceinline__ void merge64(uint64_t& a, uint64_t reversed, int lane) {
@@ -162,7 +162,9 @@ __device__ __forceinline__ bool sort_gathered(uint64_t* lists, const int* taken,
     if (count > 64) return false;
     if (wave == 0) {
         uint64_t v = lane < count ? lists[lane] : 0;
-        sort64(v, lane);
+        if (count <= 8) sort64<2, 8>(v, lane);
+        else if (count <= 32) sort64<2, 32>(v, lane);
+        else sort64(v, lane);
         lists[lane] = v;
     }
     __syncthreads();
@@ -359,12 +361,24 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(const T* __restric
         const int v_edge = edge ? v0 : v_first;
         if (v_edge >= end || (edge == 0 && v_first >= whole0)) continue;
         constexpr uint32_t kNone = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
+        const lp_u4 none{kNone, kNone, kNone, kNone};
         lp_u4 raw[kLpLoads];
+        const bool some = whole0 < (row.skew + vocab) / kPer;  // there is a load that the row fills, which lanes without one ask for
+#pragma unroll
+        for (int j = 0; j < kLpLoads; j++) {
+            const int v = v_edge + j * 64 + lane;
+            raw[j] = some ? *(const lp_u4*)(row.aligned + (int64_t)(v < end && row.whole(v) ? v : whole0) * kPer) : none;
+        }
+#pragma unroll
+        for (int j = 0; j < kLpLoads; j++) {
+            const int v = v_edge + j * 64 + lane;
+            if (v >= end || !row.whole(v)) raw[j] = none;
+        }
 #pragma unroll 1
         for (int j = 0; j < kLpLoads; j++) {
             const int v = v_edge + j * 64 + lane;
-            lp_u4 one{kNone, kNone, kNone, kNone};
-            if (v < end) one = row.whole(v) ? *(const lp_u4*)(row.aligned + (int64_t)v * kPer) : row.edge(v);
+            if (v >= end || row.whole(v)) continue;
+            const lp_u4 one = row.edge(v);
 #pragma unroll
             for (int i = 0; i < kLpLoads; i++) raw[i] = i == j ? one : raw[i];
         }

@@ -16,7 +16,7 @@
 //
 // What bounds it: with many rows the loads (a row is read once; the chosen runs again, from L2).  With few, the way through two launches: parts of a row go to several workgroups until
 // they are enough for the part, and one workgroup a row joins them (lp_plan).  1021 rows of 128256 bf16, 5 alternatives:
-// 65 us, 4.0 TB/s, vector units busy 0.85 of the time; 200 rows fp32 22 us, 4.6 TB/s; one row, 20 alternatives: 12.6 us.
+// 64 us, 4.1 TB/s, vector units busy 0.86 of the time; 200 rows fp32 22 us, 4.6 TB/s; one row, 20 alternatives: 12.6 us.
 #include <algorithm>
 
 #include "experts.h"

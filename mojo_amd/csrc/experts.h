@@ -88,7 +88,7 @@ hipError_t launch_experts_rows(const ExpertCall& c, const Routing& r, void* out,
 bool experts_gemm_supported(const ExpertCall& c, const Routing& r);
 int64_t experts_gemm_workspace_bytes(const ExpertCall& c);
 hipError_t launch_experts_gemm(const ExpertCall& c, const Routing& r, void* out, bool out_bf16, void* workspace, hipStream_t s);
-// experts_small.hip: a few rows for each expert; the sum: one token
+// experts_small.hip: a few rows for each expert; the sum: one token, or a few that hardly share an expert
 bool experts_small_wanted(const ExpertCall& c, const Routing& r);
 hipError_t launch_experts_small(const ExpertCall& c, const Routing& r, void* out, bool out_bf16, hipStream_t s);
 bool experts_sum_small_wanted(const ExpertCall& c, const Routing& r);

@@ -4,7 +4,7 @@
 // every pair is a group and nothing is looked up.  What bounds it is the way to the first product and then the weights, as in the kernel that it is made of:
 // one bf16 token, 8 of 64, 1024 x 2048 Q4_K gate and up 6.9 us (18.9 MB; 4 us to the first product); 16 fp32 tokens, 2 of 8, 14336 x 4096 Q5_K 75 us, 4.7 TB/s.
 //
-// The weighted sum of a token whose experts all have rows of their own is a product too: the experts' super-blocks one after the other as one long K, each times its expert's weight, so that one launch ends
+// The weighted sum of a token is a product too: the experts' super-blocks one after the other as one long K, each times its expert's weight, so that one launch ends
 // with the token's results (a second launch, for the sum, is 2.5 us and the pairs' results written and read).
 #include <math.h>
 
@@ -145,7 +145,15 @@ hipError_t launch_experts_small(const ExpertCall& c, const Routing& r, void* out
     }
 }
 
-bool experts_sum_small_wanted(const ExpertCall& c, const Routing& r) { return es_takes(c) && r.pairs == r.top && (c.k + 255) / 256 * r.top / kSmallWaves < 0x1fff; }
+// One token, and a few that hardly share an expert (each reads the weights of its own): the share of the pairs that a router without preference sends to different experts.  us, products and sum / this, bf16 rows, Q4_K:
+// 8 of 64, 2048 x 1024 2 tokens (0.94) 13.5 / 9.0, 4 (0.83) 15.7 / 11.8, 8 (0.66) 19.0 / 17.0; 2 of 128, 1536 x 1536 8 (0.95) 13.1 / 7.6; 4 of 16, 2048 x 1536 4 (0.68) 13.7 / 9.6; 2 of 8, 4096 x 14336 2 (0.88) 34.3 / 32.4,
+// 3 (0.77) 49.1 / 52.7; 8 of 60, 7784 x 1024 4 (0.82) 31.1 / 30.0, 6 (0.72) 36.2 / 45.7.
+bool experts_sum_small_wanted(const ExpertCall& c, const Routing& r) {
+    if (!es_takes(c) || (c.k + 255) / 256 * r.top / kSmallWaves >= 0x1fff) return false;
+    if (r.pairs == r.top) return true;
+    const double share = es_with(r) / r.pairs;
+    return share >= 0.8 || (share >= 0.6 && r.pairs * c.n * c.k <= (int64_t)48 << 20);
+}
 
 hipError_t launch_experts_sum_small(const ExpertCall& c, const Routing& r, const void* residual, int residual_dtype, void* out, bool out_bf16, hipStream_t s) {
     const SmallExperts ex{r, {c.expert_stride[0], c.expert_stride[1]}, c.lhs_top, residual, residual_dtype == QMM_BF16};

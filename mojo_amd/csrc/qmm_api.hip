@@ -1358,7 +1358,7 @@ int qmm_matmul_experts(int op, int encoding, const qmm_routing* routing, const v
     const bool out_bf16 = flags & QMM_FLAG_OUT_BF16;
     float* const y = sum ? (float*)((char*)workspace + experts_product_bytes(c)) : nullptr;
     if (sum && qmm::experts_sum_small_wanted(c, r))
-        return hip_status(qmm::launch_experts_sum_small(c, r, residual, residual_dtype, out, out_bf16, (hipStream_t)stream), "qmm_matmul_experts(sum of one token)");
+        return hip_status(qmm::launch_experts_sum_small(c, r, residual, residual_dtype, out, out_bf16, (hipStream_t)stream), "qmm_matmul_experts(sum of a few tokens)");
     void* const to = sum ? (void*)y : out;
     const bool to_bf16 = out_bf16 && !sum;
     const hipError_t e = qmm::experts_small_wanted(c, r)     ? qmm::launch_experts_small(c, r, to, to_bf16, (hipStream_t)stream)

@@ -65,7 +65,7 @@ hipError_t run_part(const ExpertCall& c, const SmallExperts& ex, int64_t groups_
 }
 template <int ENC, int MROWS, typename AT, int MODE, int EX>
 hipError_t run_small(const ExpertCall& c, const SmallExperts& ex, int64_t groups_y, int64_t expected, void* out, bool out_bf16, hipStream_t s) {
-    if constexpr (ENC == QMM_Q4_0) {
+    if constexpr (ENC == QMM_Q4_0 && MROWS < 16) {  // (es_rows: no groups of 16 rows with partial super-blocks)
         if (c.k % 256) return run_part<ENC, MROWS, AT, MODE, EX, true>(c, ex, groups_y, expected, out, out_bf16, s);
     }
     return run_part<ENC, MROWS, AT, MODE, EX, false>(c, ex, groups_y, expected, out, out_bf16, s);
@@ -87,7 +87,7 @@ int es_rows(const ExpertCall& c, const Routing& r, int64_t& expected) {
         return 1;
     }
     const double mean = es_mean(r);
-    const int rows = tokens <= 4 || mean <= 2.5 ? 4 : mean <= 6.5 || most == 8 ? 8 : 16;
+    const int rows = tokens <= 4 || mean <= 2.5 ? 4 : mean <= 6.5 || most == 8 || c.k % 256 ? 8 : 16;
     expected = std::max<int64_t>(1, (int64_t)(es_with(r) * std::max(1.0, mean / rows)));
     return rows;
 }
